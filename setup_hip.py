@@ -65,6 +65,9 @@ def build(verbose=True):
         '-DTORCH_API_INCLUDE_EXTENSION_H',
         '-DUSE_ROCM', '-D__HIP_PLATFORM_AMD__=1',
         '-fno-gpu-rdc',
+        # no packed fp32 instructions: some of their forms have given wrong
+        # results on this hardware (the host pass ignores the feature)
+        '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
         '-Wno-unused-result',
     ]
     for inc in torch_inc + [py_inc]:
