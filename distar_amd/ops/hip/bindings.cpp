@@ -961,7 +961,10 @@ void multi_clip(std::vector<torch::Tensor> grads, torch::Tensor norm_sq,
                      norm_sq.data_ptr<float>(), (float)thresh, (float)eps, 1);
 }
 
+void register_block_ops(pybind11::module_& m);   // block_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_block_ops(m);
   m.def("multi_norm_sq", &multi_norm_sq,
         "K14 multi-tensor global sum-of-squares");
   m.def("multi_clip", &multi_clip,

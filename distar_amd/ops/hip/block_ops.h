@@ -1,0 +1,74 @@
+// Host entry points of the kernels around the policy transformer. Pointers
+// are device pointers, sizes have been checked by the caller, and every call
+// only enqueues work on `stream`.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace blk {
+
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// ---- layer_norm.hip
+struct LayerNormFwd {
+  const void *x, *residual, *weight, *bias;   // residual, weight, bias: or null
+  void *y, *s;                                // s: or null without a residual
+  float *mean, *rstd;                         // or null
+  int64_t rows, x_stride, r_stride;           // strides in elements
+  int width;
+  float eps;
+};
+struct LayerNormBwd {
+  const void *dy, *ds, *s, *weight;           // ds, weight: or null
+  const float *mean, *rstd;
+  void *dx, *dweight, *dbias;                 // dweight, dbias: both or none
+  float *partial;                             // [blocks][2][width]
+  int64_t rows, dy_stride, ds_stride, s_stride;
+  int width, blocks;
+};
+int layer_norm_bwd_blocks(int64_t rows, int width, int dtype);
+void layer_norm_fwd(const LayerNormFwd&, int dtype, int wdtype, hipStream_t);
+void layer_norm_bwd(const LayerNormBwd&, int dtype, int wdtype, hipStream_t);
+
+// ---- token_logprobs.hip
+struct LogProbs {
+  const void *logits;
+  const int64_t *tokens;
+  const uint8_t *mask;                        // or null; 1: allowed
+  float *logprob, *entropy;
+  float *row_max, *row_logsum;                // or null
+  float *top_logprobs;                        // or null, [rows][top_k]
+  int64_t *top_tokens;
+  int64_t rows, stride, mask_stride, ignore_index;
+  int width, top_k;
+  float inv_temperature;
+};
+struct LogProbsBwd {
+  const void *logits;
+  const int64_t *tokens;
+  const uint8_t *mask;
+  const float *entropy, *row_max, *row_logsum;
+  const float *dlogprob, *dentropy;           // or null
+  void *dlogits;                              // contiguous
+  int64_t rows, stride, mask_stride, ignore_index;
+  int width;
+  float inv_temperature;
+};
+void token_logprobs_fwd(const LogProbs&, int dtype, hipStream_t);
+void token_logprobs_bwd(const LogProbsBwd&, int dtype, hipStream_t);
+
+// ---- grad_norm.hip
+struct GradTensor {
+  const void *in;
+  void *out;                                  // where the clipped values go
+  int64_t numel;
+  int in_dtype, out_dtype;
+};
+int64_t grad_norm_blocks(const GradTensor*, int count, int64_t* chunk);
+void grad_norm(const GradTensor*, int count, int64_t chunk, int order,
+               double* partial, int64_t blocks, float* norm, float* coef,
+               float max_norm, float eps, hipStream_t);
+void grad_scale(const GradTensor*, int count, int64_t chunk,
+                const float* coef, hipStream_t);
+
+}  // namespace blk

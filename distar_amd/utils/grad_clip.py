@@ -1,6 +1,8 @@
 """Gradient clipping strategies (reference `ctools/torch_utils/grad_clip.py:19-151`):
 none / max_norm (EMA-normalized) / momentum_norm (per-param EMA) /
-clip_value (second-moment clamp) / clip_const / pytorch_norm.
+clip_value (second-moment clamp) / clip_const / pytorch_norm, and global_norm:
+the clip of pytorch_norm for gradients of mixed types, strides and norms 1, 2
+and inf, with sums that come out the same each time (`ops/grad_norm.py`).
 
 On GPU the norm computations use torch's fused multi-tensor paths
 (`torch.nn.utils.clip_grad_norm_` with foreach=True) — one kernel per dtype
@@ -15,7 +17,7 @@ class GradClip:
     def __init__(self, clip_type, threshold=1.0, norm_type=2, begin_step=200,
                  ignore_threshold=3.0):
         assert clip_type in ('max_norm', 'clip_value', 'none', 'clip_const',
-                             'pytorch_norm', 'momentum_norm')
+                             'pytorch_norm', 'momentum_norm', 'global_norm')
         self.clip_type = clip_type
         self.threshold = threshold
         self.norm_type = norm_type
@@ -38,6 +40,10 @@ class GradClip:
                     [torch.norm(p.grad.detach(), self.norm_type) for p in params]),
                     self.norm_type)
             return total.item()
+        if self.clip_type == 'global_norm':
+            from ..ops.grad_norm import clip_grad_norm
+            return float(clip_grad_norm([p.grad for p in params], self.threshold,
+                                        self.norm_type))
         if self.clip_type == 'pytorch_norm':
             grads = [p.grad for p in params]
             if (self.norm_type == 2 and grads[0].is_cuda

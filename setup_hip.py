@@ -32,6 +32,10 @@ SOURCES = [
     os.path.join(HIP_DIR, 'residual_ln.hip'),
     os.path.join(HIP_DIR, 'conv2d.hip'),
     os.path.join(HIP_DIR, 'multi_tensor.hip'),
+    os.path.join(HIP_DIR, 'layer_norm.hip'),
+    os.path.join(HIP_DIR, 'token_logprobs.hip'),
+    os.path.join(HIP_DIR, 'grad_norm.hip'),
+    os.path.join(HIP_DIR, 'block_bindings.cpp'),
     os.path.join(HIP_DIR, 'bindings.cpp'),
 ]
 

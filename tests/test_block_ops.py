@@ -1,0 +1,496 @@
+"""Layer norm, token log probabilities and gradient clipping: the eager forms on
+the CPU, the kernels on the GPU, both against 64-bit formulas, and what they refuse.
+
+Tolerances are counted in roundings: u = 2**-24 is half a step of the 32-bit
+sums, `half(t)` half a step of a stored type.  A sum over n terms taken one after
+the other is off by at most n u times the sum of their magnitudes.
+"""
+import math
+
+import pytest
+import torch
+
+from distar_amd.ops.grad_norm import clip_grad_norm, grad_norm
+from distar_amd.ops.layer_norm import FusedLayerNorm, add_layer_norm, layer_norm
+from distar_amd.ops.token_logprobs import token_logprobs
+from distar_amd.utils.grad_clip import GradClip
+
+U = 2.0 ** -24
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def near(got, want, tol):
+    """|got - want| <= tol + the rounding of the result to its type."""
+    tol = tol + half(got.dtype) * want.abs() * 1.01 + torch.finfo(got.dtype).tiny
+    off = (got.double() - want).abs()
+    assert got.shape == want.shape
+    assert bool((off <= tol).all()), (off / tol).max()
+
+
+# ------------------------------------------------------------------ layer norm
+
+def _ln_reference(s, w, b, eps, dy=None, ds=None):
+    s, w, b = (t.double() for t in (s, w, b))
+    mean, var = s.mean(-1, keepdim=True), s.var(-1, unbiased=False, keepdim=True)
+    r = 1 / torch.sqrt(var + eps)
+    h = (s - mean) * r
+    out = {'y': h * w + b, 'h': h, 'r': r}
+    if dy is not None:
+        g = dy.double() * w
+        out['dx'] = r * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
+        if ds is not None:
+            out['dx'] = out['dx'] + ds.double()
+        flat = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+        out['dw'], out['db'] = flat(dy.double() * h).sum(0), flat(dy.double()).sum(0)
+        out['dw_abs'] = flat((dy.double() * h).abs()).sum(0)
+        out['db_abs'] = flat(dy.double().abs()).sum(0)
+    return out
+
+
+def _ln_check(x, r, w, b, dy, ds, eps=1e-5):
+    leaves = [t.clone().requires_grad_() if t is not None else None for t in (x, r, w, b)]
+    if r is None:
+        y, s = layer_norm(leaves[0], leaves[2], leaves[3], eps), x
+        grads = torch.autograd.grad(y, [leaves[0], leaves[2], leaves[3]], dy)
+    else:
+        y, s = add_layer_norm(*leaves, eps)
+        assert torch.equal(s, x + r)
+        grads = torch.autograd.grad([y, s], leaves, [dy, ds])
+        assert torch.equal(grads[0], grads[1])
+        grads = grads[1:]
+    ref = _ln_reference(s.detach(), w, b, eps, dy, ds)
+    # a mean over C values by lanes and a tree, the difference, 1/sqrt, two products
+    n = 32 + x.shape[-1] / 64
+    top, wmax = (s.detach().double().abs() * ref['r']).amax(-1, keepdim=True), w.double().abs().max()
+    near(y, ref['y'], n * U * (top * wmax * 2 + b.double().abs().max()))
+    g = (dy.double() * w.double()).abs().amax(-1, keepdim=True)
+    tol = n * U * 4 * ref['r'] * g * (1 + top * top)
+    if r is not None and x.device.type == 'cpu':
+        # autograd adds the two gradients of the stream after rounding each to its type
+        tol = tol + half(x.dtype) * ((ref['dx'] - ds.double()).abs() + ds.double().abs()) * 1.01
+    near(grads[0], ref['dx'], tol)
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    hmax = top.max() if top.numel() else 0.
+    near(grads[1], ref['dw'], (n + rows) * U * (ref['dw_abs'] + 2 * hmax * ref['db_abs']))
+    near(grads[2], ref['db'], (n + rows) * U * ref['db_abs'])
+    with torch.no_grad():
+        again = layer_norm(x, w, b, eps) if r is None else add_layer_norm(x, r, w, b, eps)[0]
+    assert torch.equal(again, y.detach())
+    return y, grads
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,width', [(1, 1), (3, 2), (5, 7), (33, 64), (70, 65), (129, 256),
+                                        (40, 257), (9, 1000), (301, 997), (7, 2049), (3, 5001),
+                                        (2, 16383), (3, 16390), (5, 20001)])
+def test_layer_norm(device, dtype, rows, width):
+    gen = torch.Generator().manual_seed(rows * 31 + width)
+    make = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, r, dy, ds = ((make(rows, width) * 2 + 0.5).to(device, dtype) for _ in range(4))
+    for residual in (False, True):
+        for wdtype in {dtype, torch.float32}:
+            w, b = (1 + 0.2 * make(width)).to(device, wdtype), make(width).to(device, wdtype)
+            _ln_check(x, r if residual else None, w, b, dy, ds if residual else None)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_layer_norm_far_mean_constant_rows_and_leading_shape(device):
+    x = torch.randn(2, 3, 4, 320) + 1000.
+    x[0, 1] = 7.
+    dy, w, b = torch.randn(2, 3, 4, 320), torch.randn(320), torch.randn(320)
+    _ln_check(*(t.to(device) if t is not None else None for t in (x, None, w, b, dy, None)))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_layer_norm_strided_rows(device, dtype):
+    big = torch.randn(12, 6, 300).to(device, dtype)
+    w, b = torch.randn(96).to(device), torch.randn(96).to(device)
+    for x in (big[:, :, 5:101], big[:, 2, 1:97], big[1, 0, 3:99], big.transpose(0, 1)[..., :96],
+              big[..., ::3][..., :96], big[:, :1, :96].expand(12, 6, 96)):
+        dy = torch.randn(x.shape).to(device, dtype)
+        want = layer_norm(x.contiguous(), w, b)
+        assert torch.equal(layer_norm(x, w, b), want)
+        leaf = x.detach().requires_grad_()
+        got, = torch.autograd.grad(layer_norm(leaf, w, b), leaf, dy[:1].expand(x.shape))
+        plain = x.contiguous().requires_grad_()
+        ref, = torch.autograd.grad(layer_norm(plain, w, b), plain, dy[:1].expand(x.shape).contiguous())
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_layer_norm_empty_partial_gradients_and_module(device):
+    w, b = torch.randn(8, device=device, requires_grad=True), torch.randn(8, device=device, requires_grad=True)
+    x = torch.zeros(0, 8, device=device, requires_grad=True)
+    y = layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y.sum(), [x, w, b])
+    assert gx.shape == (0, 8) and not gw.any() and not gb.any()
+    x = torch.randn(5, 8, device=device, requires_grad=True)
+    r = torch.randn(5, 8, device=device)
+    torch.testing.assert_close(layer_norm(x), torch.nn.functional.layer_norm(x, (8,)))
+    for weight, bias in ((w, None), (None, b)):
+        got = torch.autograd.grad(layer_norm(x, weight, bias).square().sum(), [x, w if weight is not None else b])
+        ref = torch.autograd.grad(torch.nn.functional.layer_norm(x, (8,), weight, bias).square().sum(),
+                                  [x, w if weight is not None else b])
+        torch.testing.assert_close(got, ref, rtol=1e-4, atol=1e-4)
+    y, s = add_layer_norm(x, r, w, b)                       # the stream alone
+    torch.testing.assert_close(torch.autograd.grad(s.sum(), x)[0], torch.ones_like(x))
+    module, plain = FusedLayerNorm(8).to(device), torch.nn.LayerNorm(8).to(device)
+    module.load_state_dict(plain.state_dict())
+    torch.testing.assert_close(module(x), plain(x), rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(module(x, r)[0], plain(x + r), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_layer_norm_refusals(device):
+    x = torch.randn(4, 8, device=device)
+    w = torch.ones(8, device=device)
+    with pytest.raises(ValueError):
+        layer_norm(x, w[:7])
+    with pytest.raises(ValueError):
+        layer_norm(x, w, eps=-1.)
+    with pytest.raises(ValueError):
+        layer_norm(torch.zeros(4, 0, device=device))
+    with pytest.raises(ValueError):
+        layer_norm(x[0, 0])
+    with pytest.raises(TypeError):
+        layer_norm(x.long())
+    with pytest.raises(ValueError):
+        add_layer_norm(x, x[:1])
+    with pytest.raises(TypeError):
+        add_layer_norm(x, x.bfloat16())
+    with pytest.raises(ValueError):
+        FusedLayerNorm((4, 8))
+    if device == 'cuda':
+        with pytest.raises(TypeError):
+            layer_norm(x.double())
+        with pytest.raises(TypeError):
+            layer_norm(x, w, w.bfloat16())
+        with pytest.raises(TypeError):
+            layer_norm(x.bfloat16(), w.half())
+        with pytest.raises(ValueError):
+            layer_norm(x, w.cpu())
+
+
+def test_formulas_against_differences():
+    gen = torch.Generator().manual_seed(3)
+    x, r = (torch.randn(3, 6, generator=gen, dtype=torch.float64).requires_grad_() for _ in range(2))
+    w, b = (torch.randn(6, generator=gen, dtype=torch.float64).requires_grad_() for _ in range(2))
+    assert torch.autograd.gradcheck(add_layer_norm, (x, r, w, b))
+    tokens = torch.tensor([1, -100, 5])
+    mask = torch.tensor([[1, 1, 0, 1, 0, 0], [0] * 6, [1] * 6]).bool()
+    assert torch.autograd.gradcheck(
+        lambda t: token_logprobs(t, tokens, mask=mask, temperature=0.7)[:2], (x,))
+
+
+# ------------------------------------------------------- token log probabilities
+
+def _lp_reference(logits, tokens, mask, temperature, top_k, ignore):
+    raw = logits.double()
+    ok = raw > -math.inf
+    if mask is not None:
+        ok = ok & mask
+        raw = torch.where(mask, raw, -math.inf)
+    some = ok.any(-1, keepdim=True)
+    x = torch.where(ok, raw, 0.) / temperature
+    logp = torch.where(ok, x - torch.where(ok, x, -math.inf).logsumexp(-1, keepdim=True), -math.inf)
+    p = logp.exp()
+    entropy = -torch.where(ok, p * torch.where(ok, logp, 0.), 0.).sum(-1)
+    at = tokens.clamp(min=0).unsqueeze(-1)
+    lp = torch.where(tokens == ignore, 0., logp.gather(-1, at).squeeze(-1))
+    order = torch.sort(raw, dim=-1, descending=True, stable=True)[1][..., :top_k]
+    tlp = logp.gather(-1, order)
+    return {'lp': lp, 'h': entropy, 'tlp': tlp, 'tt': torch.where(tlp > -math.inf, order, -1),
+            'p': p, 'logp': logp, 'ok': ok, 'some': some,
+            'range': (torch.where(ok, x, -math.inf).amax(-1) - torch.where(ok, x, math.inf).amin(-1)).clamp(min=0)
+            .nan_to_num(0., posinf=0.)}
+
+
+def _lp_check(logits, tokens, mask, temperature=1.0, top_k=0, ignore=-100):
+    ref = _lp_reference(logits, tokens, mask, temperature, top_k, ignore)
+    leaf = logits.detach().requires_grad_()
+    got = token_logprobs(leaf, tokens, mask=mask, temperature=temperature, top_k=top_k)
+    # a logit's distance to the maximum is exact but for 2 roundings of up to
+    # `range`; exp, the sums and log add their own
+    off = U * (64 + 8 * ref['range'])
+    finite = ref['lp'] > -math.inf
+    assert torch.equal(finite, got.logprob > -math.inf)
+    near(got.logprob[finite], ref['lp'][finite], off[finite])
+    near(got.entropy, ref['h'], off * (1 + ref['h']))
+    if top_k:
+        assert torch.equal(got.top_tokens, ref['tt'])
+        there = ref['tt'] >= 0
+        assert bool((got.top_logprobs[~there] == -math.inf).all())
+        near(got.top_logprobs[there], ref['tlp'][there], off.unsqueeze(-1).expand_as(ref['tlp'])[there])
+    gen = torch.Generator().manual_seed(9)
+    a, b = (torch.randn(tokens.shape, generator=gen).to(logits.device) for _ in range(2))
+    d, = torch.autograd.grad([got.logprob, got.entropy], leaf, [a, b])
+    a, b = a.double().unsqueeze(-1), b.double().unsqueeze(-1)
+    g = torch.where((tokens == ignore).unsqueeze(-1), 0., a)
+    one = torch.zeros_like(ref['p']).scatter_(-1, tokens.clamp(min=0).unsqueeze(-1), 1.)
+    logp = torch.where(ref['ok'], ref['logp'], 0.)
+    h = ref['h'].unsqueeze(-1)
+    want = (g * (one - ref['p']) - b * ref['p'] * (logp + h)) / temperature
+    inside = torch.ones_like(ref['ok']) if mask is None else mask.expand(logits.shape)
+    want = torch.where(ref['some'] & inside, want, 0.)
+    near(d, want, off.unsqueeze(-1) * 4 / temperature * (g.abs() + b.abs() * (1 + h)))
+    with torch.no_grad():
+        again = token_logprobs(logits, tokens, mask=mask, temperature=temperature, top_k=top_k)
+    for x, y in zip(got, again):
+        assert x is None and y is None or torch.equal(x, y)
+    return got
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,width,top_k', [(1, 1, 1), (3, 2, 2), (5, 7, 9), (16, 327, 5), (67, 513, 0),
+                                              (9, 1000, 64), (33, 1025, 3), (3, 4097, 20), (2, 24320, 5),
+                                              (2, 33001, 32), (2, 70001, 7)])
+def test_token_logprobs(device, dtype, rows, width, top_k):
+    gen = torch.Generator().manual_seed(rows + width)
+    logits = (torch.randn(rows, width, generator=gen) * 3).to(device, dtype)
+    tokens = torch.randint(0, width, (rows,), generator=gen).to(device)
+    _lp_check(logits, tokens, None, 1.0, top_k)
+    # ragged lengths with one empty row and one row of a single token; what is
+    # masked holds the type's lowest value, infinities and NaN
+    lengths = torch.randint(1, width + 1, (rows,), generator=gen)
+    lengths[rows // 2], lengths[0] = 0, 1
+    mask = (torch.arange(width) < lengths.unsqueeze(1)).to(device)
+    tokens = (torch.rand(rows, generator=gen) * lengths).long().to(device)
+    tokens[rows // 2] = -100
+    fill = torch.tensor([torch.finfo(dtype).min, math.inf, -math.inf, math.nan], device=device).to(dtype)
+    junk = fill[torch.randint(0, 4, (rows, width), generator=gen).to(device)]
+    _lp_check(torch.where(mask, logits, junk), tokens, mask, 0.7, top_k)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width', [40, 300, 3000, 40000])
+def test_token_logprobs_ties_and_infinities(device, dtype, width):
+    gen = torch.Generator().manual_seed(width)
+    tokens = torch.zeros(4, dtype=torch.long, device=device)
+    same = torch.full((4, width), 1.5).to(device, dtype)
+    got = _lp_check(same, tokens, None, 1.0, 33)
+    assert torch.equal(got.top_tokens, torch.arange(33, device=device).expand(4, 33))
+    few = torch.randint(-2, 3, (4, width), generator=gen).to(device, dtype)
+    _lp_check(few, tokens, None, 1.3, 64)
+    holes = few.clone()
+    holes[:, ::2] = -math.inf
+    holes[1] = -math.inf                                    # a row with nothing
+    holes[2, 5:] = -math.inf                                # fewer than top_k
+    _lp_check(holes, tokens + 1, None, 1.0, 8)
+    low = torch.full((4, width), torch.finfo(dtype).min, dtype=dtype, device=device)
+    low[:, 3] = 0.
+    got = token_logprobs(low, tokens + 3, top_k=2)
+    assert torch.equal(got.logprob, torch.zeros(4, device=device))
+    assert got.top_tokens[0].tolist() == [3, 0]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('width', [40, 3000, 40000])
+def test_token_logprobs_bad_rows_and_tokens(device, width):
+    logits = torch.randn(5, width, device=device)
+    logits[1, width - 1] = math.nan
+    logits[2, 7] = math.inf
+    tokens = torch.tensor([0, 0, 0, width, -1], device=device)
+    leaf = logits.requires_grad_()
+    got = token_logprobs(leaf, tokens, top_k=3)
+    assert torch.isnan(got.logprob).tolist() == [False, True, True, True, True]
+    assert torch.isnan(got.entropy).tolist() == [False, True, True, False, False]
+    assert got.top_tokens[1].tolist() == got.top_tokens[2].tolist() == [-1] * 3
+    assert bool(torch.isnan(got.top_logprobs[1:3]).all())
+    d, = torch.autograd.grad(got.logprob[0], leaf)
+    assert bool(torch.isfinite(d[0]).all()) and d[0].abs().sum() > 0
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_token_logprobs_shapes_masks_and_strides(device):
+    gen = torch.Generator().manual_seed(4)
+    big = torch.randn(3, 4, 50, generator=gen).to(device)
+    logits, tokens = big[:, :, 3:40], torch.randint(0, 37, (3, 4), generator=gen).to(device)
+    for shape in ((37,), (1, 1, 37), (3, 1, 37), (1, 4, 37), (3, 4, 37)):
+        mask = (torch.rand(shape, generator=gen) < 0.6).to(device)
+        _lp_check(logits, tokens, mask, 1.0, 4)
+    _lp_check(big.transpose(0, 1)[..., :37], tokens.t(), None, 1.0, 4)
+    _lp_check(big[..., ::2], tokens.clamp(max=24), None, 1.0, 4)
+    _lp_check(big[0, 0], torch.tensor(7, device=device), None, 1.0, 4)
+    got = token_logprobs(torch.zeros(0, 9, device=device, requires_grad=True),
+                         torch.zeros(0, dtype=torch.long, device=device), top_k=3)
+    assert got.logprob.shape == (0,) and got.top_tokens.shape == (0, 3)
+    leaf = big.clone().requires_grad_()
+    lp, h = token_logprobs(leaf, torch.zeros(3, 4, dtype=torch.int32, device=device))[:2]
+    both, = torch.autograd.grad(lp.sum() + h.sum(), leaf, retain_graph=True)
+    one, = torch.autograd.grad(lp.sum(), leaf, retain_graph=True)
+    two, = torch.autograd.grad(h.sum(), leaf)
+    torch.testing.assert_close(both, one + two, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_token_logprobs_refusals(device):
+    logits, tokens = torch.randn(4, 9, device=device), torch.zeros(4, dtype=torch.long, device=device)
+    for bad in (dict(top_k=-1), dict(top_k=65), dict(temperature=0.), dict(temperature=math.nan),
+                dict(mask=torch.ones(4, 8, device=device).bool())):
+        with pytest.raises(ValueError):
+            token_logprobs(logits, tokens, **bad)
+    with pytest.raises(ValueError):
+        token_logprobs(logits, tokens[:3])
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(4, 0, device=device), tokens)
+    with pytest.raises(TypeError):
+        token_logprobs(logits, tokens.float())
+    with pytest.raises(TypeError):
+        token_logprobs(logits, tokens, mask=torch.ones(4, 9, device=device))
+    with pytest.raises(TypeError):
+        token_logprobs(logits.long(), tokens)
+    if device == 'cuda':
+        with pytest.raises(TypeError):
+            token_logprobs(logits.double(), tokens)
+        with pytest.raises(ValueError):
+            token_logprobs(logits, tokens.cpu())
+
+
+# ------------------------------------------------------------- gradient clipping
+
+def _grads(device, gen, types, sizes=(1, 3, 1000, 0, 70001, 16385, 256)):
+    flat = torch.randn(sum(sizes) + 5, generator=gen)
+    out, at = [], 0
+    for i, n in enumerate(sizes):
+        t = types[i % len(types)]
+        out.append(flat[at:at + n].to(device, t))
+        at += n
+    buffer = torch.randn(999, generator=gen).to(device)
+    out += [buffer[1:8], buffer[8:501], buffer[501:900].view(19, 21).t()]     # views, one of them transposed
+    out.append(torch.randn((), generator=gen).to(device))
+    out.append(torch.randn(6, 5, 4, 3, generator=gen).to(device, types[-1]).contiguous(memory_format=torch.channels_last))
+    return out
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('norm_type', [1, 2, 2.0, math.inf])
+@pytest.mark.parametrize('types', [TYPES[:1], TYPES[1:2], TYPES])
+def test_clip_grad_norm(device, norm_type, types):
+    gen = torch.Generator().manual_seed(1)
+    grads = _grads(device, gen, types)
+    flat = torch.cat([g.double().reshape(-1) for g in grads])
+    want = torch.linalg.vector_norm(flat, float(norm_type))
+    # 64-bit sums, one rounding of the norm
+    near(grad_norm(grads, norm_type), want, 2 * U * want)
+    for max_norm in (1e9, float(want) * 0.37, 0.):
+        scale = min(1., max_norm / (float(want) + 1e-6))
+        copies = [g.clone(memory_format=torch.preserve_format) for g in grads]
+        norm = clip_grad_norm(copies, max_norm, norm_type)
+        near(norm, want, 2 * U * want)
+        for c, g in zip(copies, grads):
+            near(c, g.double() * scale, 8 * U * g.double().abs() * scale)
+            assert scale < 1 or torch.equal(c, g)
+        out = [torch.full_like(g, math.nan, dtype=torch.float32) for g in grads]
+        out[2] = out[2].bfloat16()
+        keep = [g.clone() for g in grads]
+        assert torch.equal(clip_grad_norm(grads, max_norm, norm_type, out=out), norm)
+        for o, g, k in zip(out, grads, keep):
+            near(o, g.double() * scale, 8 * U * g.double().abs() * scale)
+            assert torch.equal(g, k)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_clip_grad_norm_many_strided_and_neighbours(device):
+    gen = torch.Generator().manual_seed(2)
+    sizes = [1 + (37 * i) % 400 for i in range(700)]
+    flat = torch.randn(sum(sizes) + 700, generator=gen).to(device)
+    grads, at = [], 0
+    for n in sizes:                                          # one element between neighbours
+        grads.append(flat[at:at + n])
+        at += n + 1
+    before, want = flat.clone(), torch.linalg.vector_norm(torch.cat(grads).double())
+    near(clip_grad_norm(grads, 1.0), want, 2 * U * want)
+    scale = 1 / (float(want) + 1e-6)
+    gaps = torch.ones_like(flat, dtype=torch.bool)
+    at = 0
+    for n in sizes:
+        gaps[at:at + n] = False
+        at += n + 1
+    assert torch.equal(flat[gaps], before[gaps])
+    near(flat[~gaps], before[~gaps].double() * scale, 8 * U * before[~gaps].double().abs() * scale)
+    wide = torch.randn(40, 30, generator=gen).to(device)
+    kept = wide.clone()
+    part = wide[:, 3:17:2]
+    want = torch.linalg.vector_norm(part.double())
+    near(clip_grad_norm([part], 0.5), want, 2 * U * want)
+    near(part, kept[:, 3:17:2].double() * (0.5 / (float(want) + 1e-6)), 8 * U * kept[:, 3:17:2].double().abs())
+    wide[:, 3:17:2] = kept[:, 3:17:2]
+    assert torch.equal(wide, kept)
+    out = torch.zeros(7, 40, device=device).t()              # another order than its input's
+    clip_grad_norm([part], 1e9, out=[out])
+    assert torch.equal(out, part)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_clip_grad_norm_extremes(device):
+    big = [torch.full((1000,), 1e30, device=device), torch.full((3,), -1e37, device=device)]
+    want = torch.linalg.vector_norm(torch.cat(big).double())
+    near(clip_grad_norm(big, 1.0), want, 2 * U * want)
+    assert bool(torch.isfinite(big[0]).all()) and big[1][0] < 0
+    small = [torch.full((100,), 1e-30, device=device)]       # squares below the smallest 32-bit value
+    near(grad_norm(small), torch.tensor(1e-29, dtype=torch.float64, device=device), 4 * U * 1e-29)
+    for norm_type in (1, 2, math.inf):
+        for value in (math.nan, math.inf):
+            g = [torch.ones(300, device=device), torch.ones(5, device=device)]
+            g[0][211] = value
+            norm = clip_grad_norm(g, 1.0, norm_type)
+            if math.isnan(value):
+                assert torch.isnan(norm) and bool(torch.isnan(g[1]).all())
+            else:
+                assert norm == math.inf and not g[1].any() and torch.isnan(g[0][211])
+    zero = [torch.zeros(10, device=device)]
+    assert clip_grad_norm(zero, 1.0) == 0 and not zero[0].any()
+    assert grad_norm([torch.zeros(0, device=device)]) == 0
+    assert grad_norm(torch.full((4,), 2., device=device)) == 4
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_clip_grad_norm_refusals(device):
+    g = torch.ones(10, device=device)
+    for bad in (lambda: grad_norm([]), lambda: grad_norm([g], 3), lambda: clip_grad_norm([g], -1.),
+                lambda: clip_grad_norm([g], math.nan), lambda: clip_grad_norm([g], 1., eps=-1.),
+                lambda: clip_grad_norm([g], 1., out=[g, g]), lambda: clip_grad_norm([g], 1., out=[g[:9]])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        grad_norm([g.long()])
+    with pytest.raises(TypeError):
+        clip_grad_norm([g], 1., out=[g.long()])
+    if device == 'cuda':
+        with pytest.raises(TypeError):
+            grad_norm([g.double()])
+        with pytest.raises(ValueError):
+            grad_norm([g, g.cpu()])
+        for bad in ([g, g], [g[:6], g[5:]], [g[5:], g[:6]]):
+            with pytest.raises(ValueError):
+                clip_grad_norm(bad, 1.)
+        with pytest.raises(ValueError):
+            clip_grad_norm([g[:5], g[5:]], 1., out=[g[5:], torch.empty(5, device=device)])
+        with pytest.raises(ValueError):
+            clip_grad_norm([torch.ones(3, device=device)], 1., out=[torch.zeros(1, device=device).expand(3)])
+    assert torch.equal(g, torch.ones(10, device=device))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_grad_clip_global_norm_type(device):
+    gen = torch.Generator().manual_seed(6)
+    params = [torch.nn.Parameter(torch.zeros(n, device=device, dtype=t)) for n, t in ((40, torch.float32), (77, torch.bfloat16))]
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=gen).to(device, p.dtype)
+    want = torch.linalg.vector_norm(torch.cat([p.grad.double() for p in params]))
+    kept = [p.grad.clone() for p in params]
+    norm = GradClip('global_norm', threshold=1.0).apply(params)
+    assert abs(norm - float(want)) <= 2 * U * float(want)
+    for p, k in zip(params, kept):
+        near(p.grad, k.double() / (float(want) + 1e-6), 8 * U * k.double().abs())
+    assert GradClip('global_norm', threshold=1.0, norm_type=float('inf')).apply(params) <= 1.0
+    assert GradClip('global_norm').apply([torch.nn.Parameter(torch.zeros(3))]) == 0.
