@@ -325,6 +325,165 @@ Tensor token_logprobs_bwd(Tensor logits, Tensor tokens, OptTensor mask,
   return dlogits;
 }
 
+// ----------------------------------------------------------- linear layers
+
+int linear_dtype(const Tensor& t, const char* name) {
+  const int d = dtype_of(t, name);
+  TORCH_CHECK_TYPE(d != blk::kF32, name, " must be bfloat16 or float16, not float32");
+  return d;
+}
+
+void run_product(blk::Product& a, int dtype, const Tensor& like) {
+  TORCH_CHECK_VALUE(a.i <= (int64_t)1 << 30 && a.j <= (int64_t)1 << 22,
+                    "a product of ", a.i, " by ", a.j, " is too large");
+  a.splits = blk::product_splits(a);
+  Tensor partial;
+  if (a.splits > 1) {
+    partial = torch::empty({a.splits, a.i, a.j}, like.options().dtype(torch::kFloat32));
+    a.partial = partial.data_ptr<float>();
+  }
+  blk::product(a, dtype, stream_of(like));
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+// -> y, z (empty without `save`)
+std::vector<Tensor> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
+                                   OptTensor residual, int64_t act, bool save) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be on a GPU");
+  check_width(x, "x");
+  const int dtype = linear_dtype(x, "x");
+  check_device(weight, x, "weight");
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), "weight must be of x's type");
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1,
+                    "weight must be (outputs, ", x.size(-1), ")");
+  const int64_t n = weight.size(0);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = n;
+  if (bias.has_value()) {
+    check_device(*bias, x, "bias");
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == n, "bias must have ", n, " elements");
+    TORCH_CHECK_TYPE(bias->scalar_type() == x.scalar_type() ||
+                         bias->scalar_type() == torch::kFloat32,
+                     "bias must be float32 or of x's type");
+  }
+  if (residual.has_value()) {
+    check_device(*residual, x, "residual");
+    TORCH_CHECK_TYPE(residual->scalar_type() == x.scalar_type(), "residual must be of x's type");
+    TORCH_CHECK_VALUE(residual->sizes() == c10::IntArrayRef(shape),
+                      "residual must be of the output's shape");
+  }
+  const c10::DeviceGuard guard(x.device());
+  const Rows xr = rows_of(x), wr = rows_of(weight);
+  if (bias.has_value()) bias = bias->contiguous();
+  const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
+  Tensor y = torch::empty(shape, x.options());
+  Tensor z = torch::empty(save ? shape : std::vector<int64_t>{0}, x.options());
+  if (xr.rows) {
+    blk::Product a{};
+    a.p = xr.t.data_ptr();
+    a.q = wr.t.data_ptr();
+    a.p_stride = xr.stride;
+    a.q_stride = wr.stride;
+    a.i = xr.rows;
+    a.j = n;
+    a.r = x.size(-1);
+    a.out = y.data_ptr();
+    a.bias = ptr(bias);
+    a.bias_f32 = bias.has_value() && bias->scalar_type() == torch::kFloat32;
+    a.residual = residual.has_value() ? rr.t.data_ptr() : nullptr;
+    a.residual_stride = rr.stride;
+    a.z = save ? z.data_ptr() : nullptr;
+    a.act = (int)act;
+    run_product(a, dtype, x);
+  }
+  return {y, z};
+}
+
+// saved: z, or y of a relu; -> dx, dweight, dbias (empty where not needed)
+std::vector<Tensor> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, OptTensor saved,
+                                   int64_t act, bool need_x, bool need_w, bool need_b,
+                                   torch::ScalarType weight_type,
+                                   torch::ScalarType bias_type) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be on a GPU");
+  const int dtype = linear_dtype(x, "x");
+  const int64_t n = weight.size(0), k = weight.size(1);
+  check_device(dy, x, "dy");
+  check_device(weight, x, "weight");
+  TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type() &&
+                       weight.scalar_type() == x.scalar_type(),
+                   "dy and weight must be of x's type");
+  TORCH_CHECK_VALUE(x.size(-1) == k && dy.size(-1) == n && dy.numel() / n == x.numel() / k,
+                    "dy, x and weight do not fit together");
+  TORCH_CHECK_VALUE(act == blk::kNone || (saved.has_value() && saved->is_contiguous() &&
+                                          saved->numel() == dy.numel() &&
+                                          saved->scalar_type() == x.scalar_type()),
+                    "the forward pass's values are missing");
+  const c10::DeviceGuard guard(x.device());
+  const Rows yr = rows_of(dy), xr = rows_of(x), wr = rows_of(weight);
+  const int64_t rows = xr.rows;
+  Tensor dx = torch::empty(need_x ? x.sizes().vec() : std::vector<int64_t>{0}, x.options());
+  Tensor dw = torch::empty({need_w ? n : 0, k}, x.options().dtype(weight_type));
+  Tensor db = torch::empty({need_b ? n : 0}, x.options().dtype(bias_type));
+  if (!rows) {
+    dw.zero_();
+    db.zero_();
+    return {dx, dw, db};
+  }
+  const hipStream_t stream = stream_of(x);
+  Tensor dz = yr.t;
+  int64_t dz_stride = yr.stride;
+  if (act || need_b) {
+    blk::ActBwd b{};
+    b.blocks = blk::act_bwd_blocks(rows, n);
+    Tensor partial = torch::empty({need_b ? b.blocks * n : 0},
+                                  x.options().dtype(torch::kFloat32));
+    b.dy = yr.t.data_ptr();
+    if (act) {
+      dz = torch::empty({rows, n}, x.options());
+      dz_stride = n;
+      b.z = saved->data_ptr();
+      b.dz = dz.data_ptr();
+    }
+    b.partial = need_b ? partial.data_ptr<float>() : nullptr;
+    b.dbias = need_b ? db.data_ptr() : nullptr;
+    b.dbias_f32 = bias_type == torch::kFloat32;
+    b.rows = rows;
+    b.n = n;
+    b.dy_stride = yr.stride;
+    b.act = (int)act;
+    blk::act_bwd(b, dtype, stream);
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  }
+  if (need_x) {
+    blk::Product a{};
+    a.p = dz.data_ptr();
+    a.q = wr.t.data_ptr();
+    a.p_stride = dz_stride;
+    a.q_stride = wr.stride;
+    a.i = rows;
+    a.j = k;
+    a.r = n;
+    a.q_t = true;
+    a.out = dx.data_ptr();
+    run_product(a, dtype, x);
+  }
+  if (need_w) {
+    blk::Product a{};
+    a.p = dz.data_ptr();
+    a.q = xr.t.data_ptr();
+    a.p_stride = dz_stride;
+    a.q_stride = xr.stride;
+    a.i = n;
+    a.j = k;
+    a.r = rows;
+    a.p_t = a.q_t = true;
+    a.out = dw.data_ptr();
+    a.out_f32 = weight_type == torch::kFloat32;
+    run_product(a, dtype, x);
+  }
+  return {dx, dw, db};
+}
+
 // ----------------------------------------------------------- gradient norm
 
 struct Span {
@@ -437,6 +596,9 @@ void register_block_ops(pybind11::module_& m) {
   m.def("token_logprobs_fwd", &token_logprobs_fwd,
         "log probabilities of tokens, entropy and top alternatives");
   m.def("token_logprobs_bwd", &token_logprobs_bwd, "token log probabilities backward");
+  m.def("linear_act_fwd", &linear_act_fwd,
+        "linear layer with bias, activation and residual (MFMA)");
+  m.def("linear_act_bwd", &linear_act_bwd, "linear layer with epilogue, backward");
   m.def("clip_grad_norm", &clip_grad_norm,
         "norm of a list of tensors, and their scaling to a largest norm");
 }

@@ -71,4 +71,39 @@ void grad_norm(const GradTensor*, int count, int64_t chunk, int order,
 void grad_scale(const GradTensor*, int count, int64_t chunk,
                 const float* coef, hipStream_t);
 
+// ---- linear_act.hip
+enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
+// out[i][j] = epilogue(sum over r of P[i][r] Q[j][r]), where an operand lies
+// with r contiguous (P[i][r] at p + i stride + r) or, `_t`, with its other
+// index contiguous (at p + r stride + i).
+struct Product {
+  const void *p, *q;
+  int64_t p_stride, q_stride;
+  int64_t i, j, r;
+  bool p_t, q_t;
+  void *out;                                  // [i][j], contiguous
+  int out_f32;                                // float32 instead of the type
+  const void *bias;                           // [j] or null
+  int bias_f32;
+  const void *residual;                       // or null
+  int64_t residual_stride;
+  void *z;                                    // what goes into act, or null
+  int act;
+  int splits;                                 // parts of r ...
+  float *partial;                             // ... [splits][i][j], or null
+};
+struct ActBwd {
+  const void *dy, *z;                         // z: or null without act
+  void *dz;                                   // or null without act
+  float *partial;                             // [blocks][n], or null
+  void *dbias;
+  int dbias_f32;
+  int64_t rows, n, dy_stride;
+  int act, blocks;
+};
+int product_splits(const Product&);
+void product(const Product&, int dtype, hipStream_t);
+int act_bwd_blocks(int64_t rows, int64_t n);
+void act_bwd(const ActBwd&, int dtype, hipStream_t);
+
 }  // namespace blk

@@ -1,0 +1,389 @@
+// Linear layers with their epilogue, and the products of their gradients.
+//
+//   z = x W^T + b,   y = act(z) + residual
+//   dz = dy act'(z), dx = dz W,  dW = dz^T x,  db = sum over rows of dz
+//
+// One kernel does the three products out[i][j] = sum_r P[i][r] Q[j][r] on the
+// matrix cores (16x16x32, 32-bit sums): an operand's r is contiguous in
+// memory, or its other index is (W for dx, both operands for dW). Tiles of 64 r
+// go through LDS as they lie in memory, in 16-byte chunks whose place in their
+// row is XORed with bits of the row, so that the reads of a wave spread over all
+// banks; an operand with r across its rows is turned by the transposing LDS
+// read. What lies beyond r's end is loaded as zero on both sides, what lies
+// beyond i or j is loaded from a valid place and not stored.
+#include "block_common.h"
+#include "block_ops.h"
+
+namespace blk {
+namespace {
+
+constexpr int kR = 64;            // r a tile
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+__device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// ---- epilogue
+
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  if constexpr (ACT == kRelu) return z < 0.f ? 0.f : z;       // keeps a NaN
+  if constexpr (ACT == kGelu) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if constexpr (ACT == kSilu) return z / (1.f + __expf(-z));
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == kRelu) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == kGelu)
+    return 0.5f * (1.f + erff(z * 0.70710678f)) +
+           z * __expf(-0.5f * z * z) * 0.3989422804f;
+  if constexpr (ACT == kSilu) {
+    const float g = 1.f / (1.f + __expf(-z));
+    return g * (1.f + z * (1.f - g));
+  }
+  return 1.f;
+}
+
+template <int N>
+__device__ __forceinline__ void apply_act(int which, float (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    v[e] = which == kRelu ? act<kRelu>(v[e])
+         : which == kGelu ? act<kGelu>(v[e])
+         : which == kSilu ? act<kSilu>(v[e]) : v[e];
+}
+
+// the values of out[i][j ... j + N), of which n exist
+template <typename T, int N>
+__device__ __forceinline__ void finish(const Product& a, int64_t i, int64_t j,
+                                       int n, float (&v)[N]) {
+  const int64_t at = i * a.j + j;
+  if (a.bias) {
+    float b[N];
+    if (a.bias_f32) load_some<float, N>((const float*)a.bias + j, n, b, 0.f);
+    else load_some<T, N>((const T*)a.bias + j, n, b, 0.f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += b[e];
+  }
+  if (a.z) store_some<T, N>((T*)a.z + at, n, v);
+  if (a.act) apply_act<N>(a.act, v);
+  if (a.residual) {
+    float r[N];
+    load_some<T, N>((const T*)a.residual + i * a.residual_stride + j, n, r, 0.f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += r[e];
+  }
+  if (a.out_f32) store_some<float, N>((float*)a.out + at, n, v);
+  else store_some<T, N>((T*)a.out + at, n, v);
+}
+
+// ---- tiles
+
+// An operand's tile in LDS: ROWS rows of CHUNKS chunks of 8 elements. With r
+// contiguous a row is one i and holds 64 r; otherwise a row is one r and holds
+// the tile's B values of i.
+template <int B, bool TR>
+struct Tile {
+  static constexpr int rows = TR ? kR : B;
+  static constexpr int chunks = TR ? B / 8 : kR / 8;
+  static constexpr int bytes = rows * chunks * 16;
+
+  // the chunk's place in its row
+  static __device__ __forceinline__ int place(int row, int chunk) {
+    if constexpr (TR)    // pairs of chunks move together: a read takes 32 bytes
+      return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
+    else
+      return chunk ^ ((row >> 1) & 7);
+  }
+
+  // 8 consecutive r from r0 + 8 (lane / 16) of i = i0 + lane % 16
+  static __device__ __forceinline__ s16x8 fragment(const char* lds, int i0,
+                                                   int r0) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (TR) {
+      // lanes 4q ... 4q + 3 of 16 fetch row q's 16 elements; lane c gets
+      // column c of the 4 rows
+      s16x4 part[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = r0 + (lane >> 4) * 8 + h * 4 + ((lane >> 2) & 3);
+        const int col = i0 + (lane & 3) * 4;
+        const char* p = lds + (row * chunks + place(row, col >> 3)) * 16 +
+                        (col & 7) * 2;
+        part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
+      }
+      return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const int row = i0 + (lane & 15);
+      const int chunk = (r0 >> 3) + (lane >> 4);
+      return *(const s16x8*)(lds + (row * chunks + place(row, chunk)) * 16);
+    }
+  }
+};
+
+// Loads of a tile into registers, each thread N chunks, and from there to LDS.
+template <typename T, int B, bool TR, int NT>
+struct Staged {
+  using L = Tile<B, TR>;
+  static constexpr int n = L::rows * L::chunks / NT;
+  s16x8 v[n];
+
+  // base: the operand; i0, r0: the tile's origin; i_end, r_end: where it ends
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t i0,
+                                       int64_t i_end, int64_t r0, int64_t r_end) {
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const int at = k * NT + threadIdx.x;
+      const int row = at / L::chunks, chunk = at % L::chunks;
+      v[k] = (s16x8)0;
+      if constexpr (TR) {
+        const int64_t r = r0 + row;
+        const int64_t some = i_end - (i0 + chunk * 8);
+        if (r < r_end) fetch(base + r * stride + i0 + chunk * 8, some, v[k]);
+      } else {
+        int64_t i = i0 + row;
+        i = i < i_end ? i : i_end - 1;
+        const int64_t some = r_end - (r0 + chunk * 8);
+        fetch(base + i * stride + r0 + chunk * 8, some, v[k]);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void fetch(const T* p, int64_t some, s16x8& o) {
+    if (some >= 8) {
+      __builtin_memcpy(&o, p, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < some) o[e] = ((const short*)p)[e];
+    }
+  }
+
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const int at = k * NT + threadIdx.x;
+      const int row = at / L::chunks, chunk = at % L::chunks;
+      *(s16x8*)(lds + (row * L::chunks + L::place(row, chunk)) * 16) = v[k];
+    }
+  }
+};
+
+// BI x BJ of the output by WI x WJ waves.
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
+__global__ __launch_bounds__(WI * WJ * 64)
+void product_kernel(Product a) {
+  constexpr int NT = WI * WJ * 64;
+  constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
+  using P = Tile<BI, PT>;
+  using Q = Tile<BJ, QT>;
+  __shared__ __attribute__((aligned(16))) char lds[P::bytes + Q::bytes];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i0 = (int64_t)blockIdx.x * BI, j0 = (int64_t)blockIdx.y * BJ;
+  const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
+  // this block's part of r, whole tiles
+  const int64_t tiles = (a.r + kR - 1) / kR;
+  const int64_t first = tiles * blockIdx.z / gridDim.z;
+  const int64_t last = tiles * (blockIdx.z + 1) / gridDim.z;
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int x = 0; x < FI; ++x)
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
+  Staged<T, BI, PT, NT> p;
+  Staged<T, BJ, QT, NT> q;
+  if (first < last) {
+    p.load((const T*)a.p, a.p_stride, i0, a.i, first * kR, a.r);
+    q.load((const T*)a.q, a.q_stride, j0, a.j, first * kR, a.r);
+  }
+  for (int64_t t = first; t < last; ++t) {
+    __syncthreads();
+    p.store(lds);
+    q.store(lds + P::bytes);
+    __syncthreads();
+    if (t + 1 < last) {
+      p.load((const T*)a.p, a.p_stride, i0, a.i, (t + 1) * kR, a.r);
+      q.load((const T*)a.q, a.q_stride, j0, a.j, (t + 1) * kR, a.r);
+    }
+#pragma unroll
+    for (int k = 0; k < kR; k += 32) {
+      s16x8 fp[FI], fq[FJ];
+#pragma unroll
+      for (int x = 0; x < FI; ++x) fp[x] = P::fragment(lds, wi + x * 16, k);
+#pragma unroll
+      for (int y = 0; y < FJ; ++y)
+        fq[y] = Q::fragment(lds + P::bytes, wj + y * 16, k);
+#pragma unroll
+      for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y)
+          acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
+    }
+  }
+  // a lane holds 4 consecutive j of one i
+#pragma unroll
+  for (int x = 0; x < FI; ++x) {
+    const int64_t i = i0 + wi + x * 16 + (lane & 15);
+    if (i >= a.i) continue;
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) {
+      const int64_t j = j0 + wj + y * 16 + (lane >> 4) * 4;
+      const int64_t left = a.j - j;
+      if (left <= 0) continue;
+      const int n = left < 4 ? (int)left : 4;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[x][y][e];
+      if (a.partial)
+        store_some<float, 4>(a.partial + (blockIdx.z * a.i + i) * a.j + j, n, v);
+      else
+        finish<T, 4>(a, i, j, n, v);
+    }
+  }
+}
+
+// the parts of r added up in their order, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void product_join_kernel(Product a) {
+  const int64_t runs = (a.j + 3) / 4;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= a.i * runs) return;
+  const int64_t i = at / runs, j = at % runs * 4;
+  const int n = a.j - j < 4 ? (int)(a.j - j) : 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    float q[4];
+    load_some<float, 4>(a.partial + (s * a.i + i) * a.j + j, n, q, 0.f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += q[e];
+  }
+  finish<T, 4>(a, i, j, n, v);
+}
+
+// ---- dz and db
+
+// 32 threads take 8 columns each, 8 rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd_kernel(ActBwd a) {
+  __shared__ float part[8][257];
+  const int t = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 256 + t * 8;
+  const int64_t left = a.n - j;
+  const int n = left < 8 ? (int)left : 8;
+  float db[8] = {};
+  if (n > 0)
+    for (int64_t i = (int64_t)blockIdx.y * 8 + group; i < a.rows;
+         i += (int64_t)gridDim.y * 8) {
+      float d[8], z[8];
+      load_some<T, 8>((const T*)a.dy + i * a.dy_stride + j, n, d, 0.f);
+      if (a.act) {
+        load_some<T, 8>((const T*)a.z + i * a.n + j, n, z, 0.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          d[e] = a.act == kRelu ? (z[e] > 0.f ? d[e] : z[e] != z[e] ? z[e] : 0.f)
+               : a.act == kGelu ? d[e] * act_slope<kGelu>(z[e])
+                                : d[e] * act_slope<kSilu>(z[e]);
+        store_some<T, 8>((T*)a.dz + i * a.n + j, n, d);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) db[e] += d[e];
+    }
+  if (!a.partial) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[group][t * 8 + e] = db[e];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col >= a.n) return;
+  float v = 0.f;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) v += part[g][threadIdx.x];
+  a.partial[blockIdx.y * a.n + col] = v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void bias_join_kernel(ActBwd a) {
+  __shared__ float lds[64][17];
+  const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
+  const int64_t c = (int64_t)blockIdx.x * 16 + lane;
+  float v = 0.f;
+  if (c < a.n)
+    for (int k = group; k < a.blocks; k += 64) v += a.partial[k * a.n + c];
+  lds[group][lane] = v;
+  __syncthreads();
+  if (group == 0 && c < a.n) {
+    for (int k = 1; k < 64; ++k) v += lds[k][lane];
+    if (a.dbias_f32) ((float*)a.dbias)[c] = v;
+    else ((T*)a.dbias)[c] = (T)v;
+  }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <typename T, bool PT, bool QT>
+void launch(const Product& a, hipStream_t stream) {
+  const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
+                  a.splits);
+  product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
+  if (a.partial)
+    product_join_kernel<T><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 4), 256)),
+                             256, 0, stream>>>(a);
+}
+
+template <typename T>
+void launch_any(const Product& a, hipStream_t stream) {
+  if (a.p_t) launch<T, true, true>(a, stream);
+  else if (a.q_t) launch<T, false, true>(a, stream);
+  else launch<T, false, false>(a, stream);
+}
+
+template <typename T>
+void launch_act_bwd(const ActBwd& a, hipStream_t stream) {
+  act_bwd_kernel<T><<<dim3((unsigned)ceil_div(a.n, 256), a.blocks), 256, 0,
+                      stream>>>(a);
+  if (a.partial)
+    bias_join_kernel<T><<<dim3((unsigned)ceil_div(a.n, 16)), 1024, 0, stream>>>(a);
+}
+
+}  // namespace
+
+int product_splits(const Product& a) {
+  const int64_t tiles = ceil_div(a.i, 128) * ceil_div(a.j, 128);
+  const int64_t deep = ceil_div(a.r, kR);
+  int64_t s = 512 / tiles;
+  s = s < deep / 4 ? s : deep / 4;
+  return s < 1 ? 1 : (int)s;
+}
+
+void product(const Product& a, int dtype, hipStream_t stream) {
+  if (dtype == kBF16) launch_any<bf16>(a, stream);
+  else launch_any<f16>(a, stream);
+}
+
+int act_bwd_blocks(int64_t rows, int64_t n) {
+  const int64_t wide = ceil_div(n, 256);
+  int64_t b = 2048 / wide;
+  b = b < 64 ? 64 : b;
+  const int64_t need = ceil_div(rows, 8);
+  return (int)(need < b ? need : b);
+}
+
+void act_bwd(const ActBwd& a, int dtype, hipStream_t stream) {
+  if (dtype == kBF16) launch_act_bwd<bf16>(a, stream);
+  else launch_act_bwd<f16>(a, stream);
+}
+
+}  // namespace blk

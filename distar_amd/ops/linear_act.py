@@ -1,0 +1,124 @@
+"""Linear layers with bias, activation and residual in one kernel.
+
+``linear_act(x, weight, bias, activation, residual)`` computes
+``act(x W^T + b) + residual`` on the matrix cores with 32-bit sums, rounded once
+when it is stored, and has a backward pass of its own.  bfloat16 and float16;
+weights and biases may be float32 masters, then the weight is cast for the call
+and both gradients come in float32.  `ops/linear_relu.py` offers the relu
+through the library's product.
+
+On a GPU the kernels in `ops/hip/linear_act.hip` run; CPU tensors (and
+``DISTAR_AMD_DISABLE_HIP=1``) take the eager composition.
+"""
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import hip_ext
+
+ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        ops = hip_ext.require()
+        w = weight.to(x.dtype)
+        # a relu's sign can be read off its output where no residual covers it
+        from_y = act == ACTIVATIONS['relu'] and residual is None
+        y, z = ops.linear_act_fwd(x, w, bias, residual, act, act != 0 and not from_y)
+        ctx.save_for_backward(x, w, None if act == 0 else y if from_y else z)
+        ctx.act = act
+        ctx.weight_type = weight.dtype
+        ctx.bias_type = weight.dtype if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, saved = ctx.saved_tensors
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        dy = dy.to(x.dtype)
+        if need_x or need_w or need_b:
+            dx, dw, db = hip_ext.require().linear_act_bwd(
+                dy, x, w, saved, ctx.act, need_x, need_w, need_b,
+                ctx.weight_type, ctx.bias_type)
+        return (dx if need_x else None, dw if need_w else None,
+                db if need_b else None, dy if need_r else None, None)
+
+
+def _eager(x, weight, bias, activation, residual):
+    wide = torch.promote_types(x.dtype, torch.float32)
+    z = x.to(wide) @ weight.to(x.dtype).to(wide).t()
+    if bias is not None:
+        z = z + bias.to(wide)
+    if activation == 'relu':
+        z = F.relu(z)
+    elif activation == 'gelu':
+        z = F.gelu(z)
+    elif activation == 'silu':
+        z = F.silu(z)
+    if residual is not None:
+        z = z + residual.to(wide)
+    return z.to(x.dtype)
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None):
+    """``act(x @ weight.T + bias) + residual``.
+
+    x: (..., K) bfloat16 or float16; weight: (N, K) and bias: (N,), or None, in
+    x's type or float32; residual: (..., N) in x's type, or None.
+    activation: None, 'relu', 'gelu' (by the error function) or 'silu'.
+    Returns (..., N) in x's type.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got '
+                         f'{activation!r}')
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'x of shape {tuple(x.shape)} does not fit a weight of shape '
+                         f'{tuple(weight.shape)}')
+    if weight.numel() == 0:
+        raise ValueError('weight is empty')
+    if not x.is_floating_point():
+        raise TypeError(f'x must be floating point, not {x.dtype}')
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f'bias has shape {tuple(bias.shape)} for {weight.shape[0]} outputs')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and t.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f'{name} is {t.dtype}, but x is {x.dtype}')
+    if residual is not None:
+        if residual.shape != (*x.shape[:-1], weight.shape[0]):
+            raise ValueError(f'residual has shape {tuple(residual.shape)} for an output of '
+                             f'{(*x.shape[:-1], weight.shape[0])}')
+        if residual.dtype != x.dtype:
+            raise TypeError(f'residual is {residual.dtype}, but x is {x.dtype}')
+    if hip_ext.maybe_ext(x) is None:
+        return _eager(x, weight, bias, activation, residual)
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearAct.apply(x, weight, bias, residual, act)
+    return hip_ext.require().linear_act_fwd(x, weight.to(x.dtype), bias, residual, act,
+                                            False)[0]
+
+
+class LinearAct(nn.Linear):
+    """`nn.Linear` (same state dict) with an activation and, when called with
+    one, a residual in the epilogue.  Under autocast it runs in autocast's type;
+    elsewhere x must be bfloat16 or float16 on a GPU."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, **kwargs):
+        super().__init__(in_features, out_features, bias=bias, **kwargs)
+        if activation not in ACTIVATIONS:
+            raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got '
+                             f'{activation!r}')
+        self.activation = activation
+
+    def forward(self, x, residual=None):
+        if torch.is_autocast_enabled(x.device.type):
+            dtype = torch.get_autocast_dtype(x.device.type)
+            x = x.to(dtype)
+            residual = None if residual is None else residual.to(dtype)
+        return linear_act(x, self.weight, self.bias, self.activation, residual)

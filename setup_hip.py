@@ -35,6 +35,7 @@ SOURCES = [
     os.path.join(HIP_DIR, 'layer_norm.hip'),
     os.path.join(HIP_DIR, 'token_logprobs.hip'),
     os.path.join(HIP_DIR, 'grad_norm.hip'),
+    os.path.join(HIP_DIR, 'linear_act.hip'),
     os.path.join(HIP_DIR, 'block_bindings.cpp'),
     os.path.join(HIP_DIR, 'bindings.cpp'),
 ]

@@ -12,6 +12,7 @@ import torch
 
 from distar_amd.ops.grad_norm import clip_grad_norm, grad_norm
 from distar_amd.ops.layer_norm import FusedLayerNorm, add_layer_norm, layer_norm
+from distar_amd.ops.linear_act import LinearAct, linear_act
 from distar_amd.ops.token_logprobs import token_logprobs
 from distar_amd.utils.grad_clip import GradClip
 
@@ -494,3 +495,213 @@ def test_grad_clip_global_norm_type(device):
         near(p.grad, k.double() / (float(want) + 1e-6), 8 * U * k.double().abs())
     assert GradClip('global_norm', threshold=1.0, norm_type=float('inf')).apply(params) <= 1.0
     assert GradClip('global_norm').apply([torch.nn.Parameter(torch.zeros(3))]) == 0.
+
+
+# ------------------------------------------------------------------ linear layers
+
+LOW = [torch.bfloat16, torch.float16]
+SLOPE = {None: lambda z: torch.ones_like(z), 'relu': lambda z: (z > 0).double(),
+         'gelu': lambda z: torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi),
+         'silu': lambda z: torch.sigmoid(z) * (1 + z * (1 - torch.sigmoid(z)))}
+ACT = {None: lambda z: z, 'relu': torch.relu, 'gelu': torch.nn.functional.gelu, 'silu': torch.nn.functional.silu}
+
+
+def _linear_check(x, w, b, act, residual, dy):
+    """Against 64 bits. A sum of K products is off by K u of their magnitudes; the
+    slope is taken at the stored z (|act''| < 1), and dz is stored once."""
+    flat = lambda t: t.double().reshape(-1, t.shape[-1])  # noqa: E731
+    leaves = [t if t is None else t.detach().requires_grad_() for t in (x, w, b, residual)]
+    y = linear_act(leaves[0], leaves[1], leaves[2], act, leaves[3])
+    grads = iter(torch.autograd.grad(y, [t for t in leaves if t is not None], dy))
+    t, k, rows = half(x.dtype), x.shape[-1], flat(x).shape[0]
+    xd, wd, dyd = flat(x), w.to(x.dtype).double(), flat(dy)
+    z = xd @ wd.t() + (0. if b is None else b.double())
+    z_off = 2 * (k + 8) * U * (xd.abs() @ wd.abs().t() + (0. if b is None else b.double().abs()))
+    want = ACT[act](z) + (0. if residual is None else flat(residual))
+    near(y.reshape(z.shape), want, 1.2 * z_off + 16 * U * (z.abs() + want.abs()))
+    dz = dyd * SLOPE[act](z)
+    dz_off = dyd.abs() * 16 * U
+    if act == 'relu':
+        dz_off = dz_off + dyd.abs() * (z.abs() <= z_off + torch.finfo(x.dtype).tiny)
+    elif act:
+        dz_off = dz_off + dyd.abs() * (z_off + t * z.abs() * 1.01 + torch.finfo(x.dtype).tiny)
+    db_off = dz_off
+    if act:
+        dz_off = dz_off + t * dz.abs() * 1.01 + torch.finfo(x.dtype).tiny
+    if x.device.type == 'cpu':          # the eager form casts weights of another type there and back
+        dz_off = dz_off + t * dz.abs()
+    n = w.shape[0]
+    near(next(grads).reshape(xd.shape), dz @ wd, dz_off @ wd.abs() + 2 * (n + 8) * U * (dz.abs() @ wd.abs()))
+    dw = next(grads)
+    assert dw.dtype == w.dtype
+    dw_off = dz_off.t() @ xd.abs() + 2 * (rows + 8) * U * (dz.abs().t() @ xd.abs())
+    if x.device.type == 'cpu':
+        dw_off = dw_off + t * (dz.t() @ xd).abs()
+    near(dw, dz.t() @ xd, dw_off)
+    if b is not None:
+        db = next(grads)
+        assert db.dtype == b.dtype
+        near(db, dz.sum(0), db_off.sum(0) + 2 * (rows + 8) * U * dz.abs().sum(0))
+    if residual is not None:
+        assert torch.equal(next(grads), dy)
+    with torch.no_grad():
+        assert torch.equal(linear_act(x, w, b, act, residual), y)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', LOW)
+@pytest.mark.parametrize('rows,k,n', [(1, 1, 1), (3, 5, 7), (1, 1024, 256), (16, 1024, 256), (17, 997, 33), (64, 64, 64),
+                                      (65, 72, 129), (130, 997, 256), (300, 128, 260), (257, 264, 520), (1000, 8, 8),
+                                      (2100, 40, 136), (129, 2056, 24)])
+def test_linear_act(device, dtype, rows, k, n):
+    gen = torch.Generator().manual_seed(rows + k + n)
+    make = lambda *s: torch.randn(*s, generator=gen).to(device, dtype)  # noqa: E731
+    x, w, b, dy, r = make(rows, k), (make(n, k) * k ** -0.5).to(dtype), make(n), make(rows, n), make(rows, n)
+    for act in (None, 'relu', 'gelu', 'silu'):
+        _linear_check(x, w, b, act, r if act in (None, 'gelu') or rows % 2 else None, dy)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', LOW)
+def test_linear_act_strides_and_master_weights(device, dtype):
+    gen = torch.Generator().manual_seed(5)
+    make = lambda *s: torch.randn(*s, generator=gen).to(device, dtype)  # noqa: E731
+    big, wide = make(4, 50, 300), make(90, 300)
+    for lo, hi in ((0, 128), (8, 136), (3, 131), (1, 98)):
+        x, w = big[..., lo:hi], wide[:, lo:hi] * (hi - lo) ** -0.5
+        dy = make(4, 50, 90)
+        _linear_check(x, w, make(90), 'relu', big[..., 5:95], dy)
+        _linear_check(x, w.float(), make(90).float(), 'silu', None, dy[:1, :1].expand(4, 50, 90))
+        _linear_check(x, w.float(), make(90), None, big[..., 5:95], make(90, 50, 4).transpose(0, 2))
+    _linear_check(big.transpose(0, 1)[..., :64], wide.t()[:70, :64], None, 'gelu', None, make(50, 4, 70))
+    _linear_check(big[0, 0], wide[:, :300], make(90), 'gelu', make(90), make(90))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_linear_act_needed_gradients_empty_and_module(device):
+    dtype = torch.bfloat16
+    x, w, b = (torch.randn(*s, device=device).to(dtype) for s in ((9, 16), (8, 16), (8,)))
+    full = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(linear_act(*full, 'gelu').float().sum(), full)
+    for i in range(3):
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(linear_act(*leaves, 'gelu').float().sum(), leaves[i])
+        assert torch.equal(got, want[i])
+    none = torch.zeros(0, 16, device=device, dtype=dtype, requires_grad=True)
+    y = linear_act(none, full[1], full[2], 'relu')
+    got = torch.autograd.grad(y.float().sum(), [none, *full[1:]])
+    assert y.shape == (0, 8) and got[0].shape == (0, 16) and not got[1].any() and not got[2].any()
+    nan = x.clone()
+    nan[4, 3] = math.nan
+    for act in (None, 'relu', 'gelu', 'silu'):
+        y = linear_act(nan, w, b, act)
+        assert bool(torch.isnan(y[4]).all()) and bool(torch.isfinite(y[[0, 1, 2, 3, 5, 6, 7, 8]]).all())
+    module = LinearAct(16, 8, activation='relu').to(device)
+    module.load_state_dict(torch.nn.Linear(16, 8).state_dict())
+    with torch.autocast(device, dtype=dtype):
+        y = module(x.float(), x[:, :8].float())
+    assert y.dtype == dtype
+    y.float().sum().backward()
+    assert module.weight.grad.dtype == torch.float32 and bool(torch.isfinite(module.weight.grad).all())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_linear_act_refusals(device):
+    x, w = torch.randn(4, 8, device=device).bfloat16(), torch.randn(3, 8, device=device).bfloat16()
+    for bad in (lambda: linear_act(x, w, activation='tanh'), lambda: linear_act(x[:, :7], w), lambda: linear_act(x, w[0]),
+                lambda: linear_act(x, w, w[0]), lambda: linear_act(x, w, residual=x), lambda: linear_act(x[0, 0], w),
+                lambda: linear_act(x, w[:0]), lambda: LinearAct(3, 4, activation='no')):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: linear_act(x, w.half()), lambda: linear_act(x.long(), w),
+                lambda: linear_act(x, w, residual=torch.zeros(4, 3, device=device))):
+        with pytest.raises(TypeError):
+            bad()
+    if device == 'cuda':
+        with pytest.raises(TypeError):
+            linear_act(x.float(), w.float())
+        with pytest.raises(ValueError):
+            linear_act(x, w.cpu())
+
+
+# ------------------------------------------------------------------ together
+
+def _block(p, x, tokens, mask, eager=None):
+    """A pre-norm sublayer, its policy head and its loss."""
+    ln, add_ln, lin = (layer_norm, add_layer_norm, linear_act) if eager is None else eager
+    h = lin(ln(x, p['w1'], p['b1']), p['up'], p['ub'], 'gelu')
+    y, s = add_ln(lin(h, p['down'], p['db'], 'relu', x), x, p['w2'], p['b2'])
+    logits = lin(y, p['head'], p['hb'])
+    lp, entropy = token_logprobs(logits, tokens, mask=mask)[:2]
+    return -(lp.clamp(min=-50.).mean()) - 0.1 * entropy.mean() + 0.01 * s.float().square().mean()
+
+
+def _block_inputs(device, dtype):
+    gen = torch.Generator().manual_seed(8)
+    make = lambda *s, scale=0.1: (torch.randn(*s, generator=gen) * scale).to(device, dtype)  # noqa: E731
+    p = {'w1': 1 + make(96), 'b1': make(96), 'up': make(200, 96), 'ub': make(200), 'down': make(96, 200), 'db': make(96),
+         'w2': 1 + make(96), 'b2': make(96), 'head': make(37, 96), 'hb': make(37)}
+    x = make(6, 11, 96, scale=1.)
+    tokens = torch.randint(0, 37, (6, 11), generator=gen)
+    mask = torch.rand(6, 11, 37, generator=gen) < 0.8
+    mask.scatter_(-1, tokens.unsqueeze(-1), True)
+    mask[2, 3], tokens[2, 3], tokens[0, 0] = False, -100, -100
+    return p, x, tokens.to(device), mask.to(device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', LOW)
+def test_block_step_together(dtype):
+    p, x, tokens, mask = _block_inputs('cuda', dtype)
+    p = {k: v.requires_grad_() for k, v in p.items()}
+    got = torch.autograd.grad(_block(p, x, tokens, mask), list(p.values()))
+    wide = {k: v.detach().cpu().double().requires_grad_() for k, v in p.items()}
+    ref = torch.autograd.grad(_block(wide, x.cpu().double(), tokens.cpu(), mask.cpu()), list(wide.values()))
+    for g, r, name in zip(got, ref, p):
+        # about ten stored values lie between the loss and a weight, each off by half
+        # a step in independent directions, and the relu's flips are of their order
+        off = torch.linalg.vector_norm(g.cpu().double() - r) / torch.linalg.vector_norm(r)
+        assert off <= 16 * half(dtype), (name, float(off))
+    master = [torch.empty_like(g, dtype=torch.float32) for g in got]
+    norm = clip_grad_norm(got, 0.01, out=master)
+    near(norm, torch.linalg.vector_norm(torch.cat([g.double().reshape(-1) for g in got])), 2 * U * norm.double())
+    assert abs(float(grad_norm(master)) - 0.01) <= 1e-6
+
+
+@pytest.mark.gpu
+def test_block_step_in_graph_and_on_another_stream():
+    def step(p, x, tokens, mask):
+        leaves = {k: v.detach().requires_grad_() for k, v in p.items()}
+        loss = _block(leaves, x, tokens, mask)
+        grads = list(torch.autograd.grad(loss, list(leaves.values())))
+        norm = clip_grad_norm(grads, 0.05)
+        return [loss.detach(), norm, *grads]
+
+    inputs = [_block_inputs('cuda', torch.bfloat16)]
+    eager = step(*inputs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(*inputs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(eager, other):
+        assert torch.equal(a, b)
+    p, x, tokens, mask = inputs[0]
+    x = x.clone()
+    graphs = []
+    for _ in range(2):                              # two graphs with workspaces of their own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(p, x, tokens, mask)
+        graphs.append((graph, out))
+    for turn in range(4):
+        x.copy_(torch.randn(x.shape, device='cuda'))
+        want = step(p, x, tokens, mask)
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
