@@ -18,20 +18,23 @@ from . import hip_ext
 _ORDERS = {1.0: 1, 2.0: 2, math.inf: 0}
 
 
-def _check(tensors, norm_type):
+def _prepare(tensors, norm_type):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError('no tensors were given')
     order = _ORDERS.get(float(norm_type))
     if order is None:
         raise ValueError(f'norm_type must be 1, 2 or inf, got {norm_type}')
+    return tensors, order
+
+
+def _check(tensors):
     for t in tensors:
         if not t.is_floating_point() or t.layout != torch.strided:
             raise TypeError(f'gradients must be dense floating point tensors, got '
                             f'{t.dtype}, {t.layout}')
         if t.device != tensors[0].device:
             raise ValueError(f'gradients are on {tensors[0].device} and {t.device}')
-    return tensors, order
 
 
 def _eager_norm(tensors, order):
@@ -49,10 +52,12 @@ def _eager_norm(tensors, order):
 def grad_norm(tensors, norm_type=2.0):
     """The norm (1, 2 or inf) over all elements of `tensors`, as a 0-d float32
     tensor on their device."""
-    tensors, order = _check(tensors, norm_type)
-    if hip_ext.maybe_ext(tensors[0]) is None:
-        return _eager_norm(tensors, order)
-    return hip_ext.require().clip_grad_norm(tensors, None, order, 0., 0., False)[0]
+    tensors, order = _prepare(tensors, norm_type)
+    ext = hip_ext.maybe_ext(tensors[0])
+    if ext is not None:
+        return ext.clip_grad_norm(tensors, None, order, 0., 0., False)
+    _check(tensors)
+    return _eager_norm(tensors, order)
 
 
 @torch.no_grad()
@@ -66,7 +71,7 @@ def clip_grad_norm(tensors, max_norm, norm_type=2.0, eps=1e-6, out=None):
     results NaN, an infinite one makes them 0 (and infinities NaN), as the
     formula says.
     """
-    tensors, order = _check(tensors, norm_type)
+    tensors, order = _prepare(tensors, norm_type)
     if not max_norm >= 0:
         raise ValueError(f'max_norm must not be negative, got {max_norm}')
     if not eps >= 0:
@@ -75,15 +80,16 @@ def clip_grad_norm(tensors, max_norm, norm_type=2.0, eps=1e-6, out=None):
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(tensors):
             raise ValueError(f'out has {len(out)} tensors for {len(tensors)}')
-        for o, t in zip(out, tensors):
-            if o.shape != t.shape:
-                raise ValueError(f'an output of shape {tuple(o.shape)} was given for '
-                                 f'{tuple(t.shape)}')
-            if not o.is_floating_point() or o.device != t.device:
-                raise TypeError(f'an output is {o.dtype} on {o.device}')
-    if hip_ext.maybe_ext(tensors[0]) is not None:
-        return hip_ext.require().clip_grad_norm(tensors, out, order, float(max_norm),
-                                                float(eps), True)[0]
+    ext = hip_ext.maybe_ext(tensors[0])
+    if ext is not None:
+        return ext.clip_grad_norm(tensors, out, order, max_norm, eps, True)
+    _check(tensors)
+    for o, t in zip(out or [], tensors):
+        if o.shape != t.shape:
+            raise ValueError(f'an output of shape {tuple(o.shape)} was given for '
+                             f'{tuple(t.shape)}')
+        if not o.is_floating_point() or o.device != t.device:
+            raise TypeError(f'an output is {o.dtype} on {o.device}')
     norm = _eager_norm(tensors, order)
     scale = (max_norm / (norm + eps)).clamp(max=1.0)
     for t, o in zip(tensors, tensors if out is None else out):

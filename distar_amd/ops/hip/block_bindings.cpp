@@ -1,13 +1,16 @@
 // Python bindings of the kernels around the policy transformer: checks of the
-// arguments, outputs and workspaces, and the launch on the current stream of
-// the tensors' own device.
+// arguments, outputs and workspaces, the launch on the current stream of the
+// tensors' own device, and the autograd nodes. The nodes are C++ so that a
+// small call costs a few microseconds on the host instead of some fifty.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
-#include <limits>
+#include <array>
+#include <cmath>
 
 #include "block_ops.h"
 
@@ -69,6 +72,28 @@ void check_width(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.size(-1) <= (1 << 30), name, " is wider than 2^30");
 }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(std::initializer_list<const OptTensor*> inputs) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const auto* t : inputs)
+    if (t->has_value() && (*t)->requires_grad()) return true;
+  return false;
+}
+
+// Gradients come without a graph of their own: where one is being built, using
+// it raises an error.
+variable_list once(variable_list grads, const char* what) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " is not differentiable twice", (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+Tensor none_or(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
 // ------------------------------------------------------------ layer norm
 
 int check_affine(const Tensor& x, const OptTensor& w, const OptTensor& b,
@@ -95,11 +120,12 @@ const void* ptr(const OptTensor& t) {
   return t.has_value() ? t->data_ptr() : nullptr;
 }
 
-// -> y, s (x itself without a residual), mean, rstd (empty without `stats`)
-std::vector<Tensor> layer_norm_fwd(Tensor x, OptTensor residual, OptTensor weight,
+// -> y, s (x itself without a residual), stats (mean, rstd; undefined if unasked)
+std::array<Tensor, 3> layer_norm_fwd(Tensor x, OptTensor residual, OptTensor weight,
                                    OptTensor bias, double eps, bool stats) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be on a GPU");
   check_width(x, "x");
+  TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative, got ", eps);
   const int dtype = dtype_of(x, "x");
   const int wdtype = check_affine(x, weight, bias, dtype);
   if (residual.has_value()) {
@@ -115,9 +141,8 @@ std::vector<Tensor> layer_norm_fwd(Tensor x, OptTensor residual, OptTensor weigh
   const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
   Tensor y = torch::empty(x.sizes(), x.options());
   Tensor s = residual.has_value() ? torch::empty(x.sizes(), x.options()) : x;
-  const auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor mean = torch::empty({stats ? xr.rows : 0}, f32);
-  Tensor rstd = torch::empty({stats ? xr.rows : 0}, f32);
+  Tensor kept;
+  if (stats) kept = torch::empty({2, xr.rows}, x.options().dtype(torch::kFloat32));
   if (xr.rows) {
     blk::LayerNormFwd a{};
     a.x = xr.t.data_ptr();
@@ -126,8 +151,8 @@ std::vector<Tensor> layer_norm_fwd(Tensor x, OptTensor residual, OptTensor weigh
     a.bias = ptr(bias);
     a.y = y.data_ptr();
     a.s = residual.has_value() ? s.data_ptr() : nullptr;
-    a.mean = stats ? mean.data_ptr<float>() : nullptr;
-    a.rstd = stats ? rstd.data_ptr<float>() : nullptr;
+    a.mean = stats ? kept.data_ptr<float>() : nullptr;
+    a.rstd = stats ? a.mean + xr.rows : nullptr;
     a.rows = xr.rows;
     a.x_stride = xr.stride;
     a.r_stride = rr.stride;
@@ -136,18 +161,14 @@ std::vector<Tensor> layer_norm_fwd(Tensor x, OptTensor residual, OptTensor weigh
     blk::layer_norm_fwd(a, dtype, wdtype, stream_of(x));
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
-  return {y, s, mean, rstd};
+  return {y, s, kept};
 }
 
-// -> dx, dweight, dbias (empty without `params`)
-std::vector<Tensor> layer_norm_bwd(Tensor dy, OptTensor ds, Tensor s, Tensor mean,
-                                   Tensor rstd, OptTensor weight, bool params,
-                                   torch::ScalarType param_type) {
-  TORCH_CHECK_VALUE(s.is_cuda(), "s must be on a GPU");
-  check_width(s, "s");
+// -> dx, dweight, dbias (the last two undefined without `params`)
+std::array<Tensor, 3> layer_norm_bwd(Tensor dy, OptTensor ds, Tensor s, Tensor stats,
+                                     OptTensor weight, bool params,
+                                     torch::ScalarType param_type) {
   const int dtype = dtype_of(s, "s");
-  const OptTensor none;
-  int wdtype = check_affine(s, weight, none, dtype);
   check_device(dy, s, "dy");
   TORCH_CHECK_VALUE(dy.sizes() == s.sizes(), "dy must be of s's shape");
   TORCH_CHECK_TYPE(dy.scalar_type() == s.scalar_type(), "dy must be of s's type");
@@ -160,41 +181,29 @@ std::vector<Tensor> layer_norm_bwd(Tensor dy, OptTensor ds, Tensor s, Tensor mea
   const Rows yr = rows_of(dy), sr = rows_of(s);
   const Rows dr = ds.has_value() ? rows_of(*ds) : Rows{s, 0, 0};
   const int64_t width = s.size(-1);
-  const auto f32 = s.options().dtype(torch::kFloat32);
-  TORCH_CHECK_VALUE(mean.is_contiguous() && mean.numel() == sr.rows &&
-                        mean.scalar_type() == torch::kFloat32 &&
-                        rstd.is_contiguous() && rstd.numel() == sr.rows &&
-                        rstd.scalar_type() == torch::kFloat32,
-                    "mean and rstd must be the forward pass's own");
-  check_device(mean, s, "mean");
-  check_device(rstd, s, "rstd");
   Tensor dx = torch::empty(s.sizes(), s.options());
-  const auto ptype = s.options().dtype(param_type);
-  Tensor dw = torch::empty({params ? width : 0}, ptype);
-  Tensor db = torch::empty({params ? width : 0}, ptype);
+  Tensor dw, db;
   if (params) {
-    const int d = dtype_of(dw, "weight or bias");
-    TORCH_CHECK_TYPE(d == dtype || d == blk::kF32,
-                     "weight and bias must be float32 or of the input's type");
-    TORCH_CHECK_TYPE(!weight.has_value() || d == wdtype,
-                     "weight and bias must be of one type");
-    wdtype = d;
+    const auto options = s.options().dtype(param_type);
+    dw = torch::empty({width}, options);
+    db = torch::empty({width}, options);
   }
   if (!sr.rows) {
-    dw.zero_();
-    db.zero_();
+    if (params) dw.zero_(), db.zero_();
     return {dx, dw, db};
   }
   if (weight.has_value()) weight = weight->contiguous();
   blk::LayerNormBwd a{};
   a.blocks = blk::layer_norm_bwd_blocks(sr.rows, (int)width, dtype);
-  Tensor partial = torch::empty({params ? a.blocks * 2 * width : 0}, f32);
+  Tensor partial;
+  if (params)
+    partial = torch::empty({a.blocks * 2 * width}, s.options().dtype(torch::kFloat32));
   a.dy = yr.t.data_ptr();
   a.ds = ds.has_value() ? dr.t.data_ptr() : nullptr;
   a.s = sr.t.data_ptr();
   a.weight = ptr(weight);
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
+  a.mean = stats.data_ptr<float>();
+  a.rstd = a.mean + sr.rows;
   a.dx = dx.data_ptr();
   a.dweight = params ? dw.data_ptr() : nullptr;
   a.dbias = params ? db.data_ptr() : nullptr;
@@ -204,9 +213,66 @@ std::vector<Tensor> layer_norm_bwd(Tensor dy, OptTensor ds, Tensor s, Tensor mea
   a.ds_stride = dr.stride;
   a.s_stride = sr.stride;
   a.width = (int)width;
-  blk::layer_norm_bwd(a, dtype, wdtype, stream_of(s));
+  blk::layer_norm_bwd(a, dtype, param_type == torch::kFloat32 ? (int)blk::kF32 : dtype,
+                      stream_of(s));
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {dx, dw, db};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  enum { kX = 1, kResidual = 2, kWeight = 4, kBias = 8 };
+
+  static variable_list forward(AutogradContext* ctx, Tensor x, OptTensor residual,
+                               OptTensor weight, OptTensor bias, double eps) {
+    const auto r = layer_norm_fwd(x, residual, weight, bias, eps, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r[1], r[2], none_or(weight)});
+    int64_t need = x.requires_grad() ? kX : 0;
+    if (residual.has_value() && residual->requires_grad()) need |= kResidual;
+    if (weight.has_value() && weight->requires_grad()) need |= kWeight;
+    if (bias.has_value() && bias->requires_grad()) need |= kBias;
+    ctx->saved_data["need"] = need;
+    ctx->saved_data["type"] = (int64_t)(weight.has_value() ? weight->scalar_type()
+                                        : bias.has_value() ? bias->scalar_type()
+                                                           : x.scalar_type());
+    if (residual.has_value()) return {r[0], r[1]};
+    return {r[0]};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const Tensor& s = saved[0];
+    const Tensor dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
+    Tensor dx = ds, dw, db;                // where only the stream was used
+    if (dy.defined()) {
+      const auto r = layer_norm_bwd(dy, opt(ds), s, saved[1], opt(saved[2]),
+                                    need & (kWeight | kBias),
+                                    (torch::ScalarType)ctx->saved_data["type"].toInt());
+      dx = r[0], dw = r[1], db = r[2];
+    }
+    return once({need & kX ? dx : Tensor(), need & kResidual ? dx : Tensor(),
+                 need & kWeight ? dw : Tensor(), need & kBias ? db : Tensor(), Tensor()},
+                "layer_norm");
+  }
+};
+
+Tensor layer_norm(Tensor x, OptTensor weight, OptTensor bias, double eps) {
+  const OptTensor leaf = x;
+  if (wants_grad({&leaf, &weight, &bias}))
+    return LayerNorm::apply(x, OptTensor(), weight, bias, eps)[0];
+  return layer_norm_fwd(x, {}, weight, bias, eps, false)[0];
+}
+
+std::pair<Tensor, Tensor> add_layer_norm(Tensor x, Tensor residual, OptTensor weight,
+                                         OptTensor bias, double eps) {
+  const OptTensor leaf = x, other = residual;
+  if (wants_grad({&leaf, &other, &weight, &bias})) {
+    const auto r = LayerNorm::apply(x, other, weight, bias, eps);
+    return {r[0], r[1]};
+  }
+  const auto r = layer_norm_fwd(x, other, weight, bias, eps, false);
+  return {r[0], r[1]};
 }
 
 // ------------------------------------------------- token log probabilities
@@ -225,21 +291,29 @@ LogitRows check_logits(const Tensor& logits, const Tensor& tokens,
   r.dtype = dtype_of(logits, "logits");
   r.logits = rows_of(logits);
   check_device(tokens, logits, "tokens");
-  TORCH_CHECK_TYPE(tokens.scalar_type() == torch::kLong, "tokens must be int64");
+  switch (tokens.scalar_type()) {
+    case torch::kLong: case torch::kInt: case torch::kShort: case torch::kByte: break;
+    default: TORCH_CHECK_TYPE(false, "tokens must be integers, not ", tokens.scalar_type());
+  }
   TORCH_CHECK_VALUE(tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                     "tokens must have the shape of logits without its last dimension");
-  r.tokens = tokens.contiguous();
+  r.tokens = tokens.to(torch::kLong).contiguous();
   if (mask.has_value()) {
     check_device(*mask, logits, "mask");
     TORCH_CHECK_TYPE(mask->scalar_type() == torch::kBool, "mask must be bool");
+    bool fits = mask->dim() <= logits.dim();
+    for (int64_t d = 1; fits && d <= mask->dim(); ++d)
+      fits = mask->size(-d) == 1 || mask->size(-d) == logits.size(-d);
+    TORCH_CHECK_VALUE(fits, "mask of shape ", mask->sizes(),
+                      " does not broadcast to logits of shape ", logits.sizes());
     r.mask = rows_of(mask->expand(logits.sizes()));
   }
   return r;
 }
 
-// -> logprob, entropy, row_max, row_logsum (both empty without `stats`),
-//    top_logprobs, top_tokens
-std::vector<Tensor> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor mask,
+// -> logprob, entropy, top_logprobs, top_tokens (both of width 0 without top_k),
+//    stats (maximum, log of the sum; undefined if unasked)
+std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor mask,
                                        double temperature, int64_t top_k,
                                        int64_t ignore_index, bool stats) {
   const c10::OptionalDeviceGuard guard(
@@ -247,16 +321,20 @@ std::vector<Tensor> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor m
   const LogitRows r = check_logits(logits, tokens, mask);
   const int64_t rows = r.logits.rows;
   const int64_t k = std::min<int64_t>(top_k, logits.size(-1));
-  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= 64, "top_k must be 0 to 64");
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= 64, "top_k must be 0 to 64, got ", top_k);
+  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature),
+                    "temperature must be positive, got ", temperature);
   const auto f32 = logits.options().dtype(torch::kFloat32);
   Tensor logprob = torch::empty(tokens.sizes(), f32);
   Tensor entropy = torch::empty(tokens.sizes(), f32);
-  Tensor row_max = torch::empty({stats ? rows : 0}, f32);
-  Tensor row_logsum = torch::empty({stats ? rows : 0}, f32);
-  std::vector<int64_t> shape = tokens.sizes().vec();
-  shape.push_back(k);
-  Tensor top_lp = torch::empty(shape, f32);
-  Tensor top_t = torch::empty(shape, logits.options().dtype(torch::kLong));
+  Tensor kept, top_lp, top_t;
+  if (stats) kept = torch::empty({2, rows}, f32);
+  if (top_k) {
+    std::vector<int64_t> shape = tokens.sizes().vec();
+    shape.push_back(k);
+    top_lp = torch::empty(shape, f32);
+    top_t = torch::empty(shape, logits.options().dtype(torch::kLong));
+  }
   if (rows) {
     blk::LogProbs a{};
     a.logits = r.logits.t.data_ptr();
@@ -264,8 +342,8 @@ std::vector<Tensor> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor m
     a.mask = mask.has_value() ? (const uint8_t*)r.mask.t.data_ptr() : nullptr;
     a.logprob = logprob.data_ptr<float>();
     a.entropy = entropy.data_ptr<float>();
-    a.row_max = stats ? row_max.data_ptr<float>() : nullptr;
-    a.row_logsum = stats ? row_logsum.data_ptr<float>() : nullptr;
+    a.row_max = stats ? kept.data_ptr<float>() : nullptr;
+    a.row_logsum = stats ? a.row_max + rows : nullptr;
     a.top_logprobs = k ? top_lp.data_ptr<float>() : nullptr;
     a.top_tokens = k ? top_t.data_ptr<int64_t>() : nullptr;
     a.rows = rows;
@@ -278,27 +356,18 @@ std::vector<Tensor> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor m
     blk::token_logprobs_fwd(a, r.dtype, stream_of(logits));
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
-  return {logprob, entropy, row_max, row_logsum, top_lp, top_t};
+  return {logprob, entropy, top_lp, top_t, kept};
 }
 
 Tensor token_logprobs_bwd(Tensor logits, Tensor tokens, OptTensor mask,
-                          Tensor entropy, Tensor row_max, Tensor row_logsum,
-                          OptTensor dlogprob, OptTensor dentropy,
-                          double temperature, int64_t ignore_index) {
-  const c10::OptionalDeviceGuard guard(
-      logits.is_cuda() ? c10::optional<c10::Device>(logits.device()) : c10::nullopt);
+                          Tensor entropy, Tensor stats, OptTensor dlogprob,
+                          OptTensor dentropy, double temperature,
+                          int64_t ignore_index) {
+  const c10::DeviceGuard guard(logits.device());
   const LogitRows r = check_logits(logits, tokens, mask);
   const int64_t rows = r.logits.rows;
-  for (const Tensor* t : {&entropy, &row_max, &row_logsum}) {
-    check_device(*t, logits, "a row's statistics");
-    TORCH_CHECK_VALUE(t->is_contiguous() && t->numel() == rows &&
-                          t->scalar_type() == torch::kFloat32,
-                      "a row's statistics must be the forward pass's own");
-  }
   for (OptTensor* t : {&dlogprob, &dentropy}) {
     if (!t->has_value()) continue;
-    check_device(**t, logits, "a gradient");
-    TORCH_CHECK_VALUE((*t)->sizes() == tokens.sizes(), "a gradient must be of tokens' shape");
     *t = (*t)->to(torch::kFloat32).contiguous();
   }
   Tensor dlogits = torch::empty(logits.sizes(), logits.options());
@@ -308,8 +377,8 @@ Tensor token_logprobs_bwd(Tensor logits, Tensor tokens, OptTensor mask,
     a.tokens = r.tokens.data_ptr<int64_t>();
     a.mask = mask.has_value() ? (const uint8_t*)r.mask.t.data_ptr() : nullptr;
     a.entropy = entropy.data_ptr<float>();
-    a.row_max = row_max.data_ptr<float>();
-    a.row_logsum = row_logsum.data_ptr<float>();
+    a.row_max = stats.data_ptr<float>();
+    a.row_logsum = a.row_max + rows;
     a.dlogprob = (const float*)ptr(dlogprob);
     a.dentropy = (const float*)ptr(dentropy);
     a.dlogits = dlogits.data_ptr();
@@ -323,6 +392,48 @@ Tensor token_logprobs_bwd(Tensor logits, Tensor tokens, OptTensor mask,
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   return dlogits;
+}
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list forward(AutogradContext* ctx, Tensor logits, Tensor tokens,
+                               OptTensor mask, double temperature, int64_t top_k,
+                               int64_t ignore_index) {
+    const auto r = token_logprobs_fwd(logits, tokens, mask, temperature, top_k,
+                                      ignore_index, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, tokens, none_or(mask), r[1], r[4]});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    if (!top_k) return {r[0], r[1]};
+    ctx->mark_non_differentiable({r[2], r[3]});
+    return {r[0], r[1], r[2], r[3]};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor d;
+    if (grads[0].defined() || grads[1].defined())
+      d = token_logprobs_bwd(saved[0], saved[1], opt(saved[2]), saved[3], saved[4],
+                             opt(grads[0]), opt(grads[1]),
+                             ctx->saved_data["temperature"].toDouble(),
+                             ctx->saved_data["ignore_index"].toInt());
+    return once({d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "token_logprobs");
+  }
+};
+
+// -> logprob, entropy, top_logprobs, top_tokens (None without top_k)
+std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(
+    Tensor logits, Tensor tokens, OptTensor mask, double temperature, int64_t top_k,
+    int64_t ignore_index) {
+  const OptTensor leaf = logits;
+  if (wants_grad({&leaf})) {
+    const auto r = LogProbs::apply(logits, tokens, mask, temperature, top_k, ignore_index);
+    if (!top_k) return {r[0], r[1], OptTensor(), OptTensor()};
+    return {r[0], r[1], r[2], r[3]};
+  }
+  const auto r = token_logprobs_fwd(logits, tokens, mask, temperature, top_k, ignore_index,
+                                    false);
+  return {r[0], r[1], opt(r[2]), opt(r[3])};
 }
 
 // ----------------------------------------------------------- linear layers
@@ -346,14 +457,16 @@ void run_product(blk::Product& a, int dtype, const Tensor& like) {
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-// -> y, z (empty without `save`)
-std::vector<Tensor> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
+// -> y, z (undefined without `save`)
+std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
                                    OptTensor residual, int64_t act, bool save) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be on a GPU");
   check_width(x, "x");
   const int dtype = linear_dtype(x, "x");
   check_device(weight, x, "weight");
-  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), "weight must be of x's type");
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type() ||
+                       weight.scalar_type() == torch::kFloat32,
+                   "weight must be float32 or of x's type");
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1,
                     "weight must be (outputs, ", x.size(-1), ")");
   const int64_t n = weight.size(0);
@@ -373,11 +486,12 @@ std::vector<Tensor> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
                       "residual must be of the output's shape");
   }
   const c10::DeviceGuard guard(x.device());
-  const Rows xr = rows_of(x), wr = rows_of(weight);
+  const Rows xr = rows_of(x), wr = rows_of(weight.to(x.scalar_type()));
   if (bias.has_value()) bias = bias->contiguous();
   const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
   Tensor y = torch::empty(shape, x.options());
-  Tensor z = torch::empty(save ? shape : std::vector<int64_t>{0}, x.options());
+  Tensor z;
+  if (save) z = torch::empty(shape, x.options());
   if (xr.rows) {
     blk::Product a{};
     a.p = xr.t.data_ptr();
@@ -399,34 +513,22 @@ std::vector<Tensor> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
   return {y, z};
 }
 
-// saved: z, or y of a relu; -> dx, dweight, dbias (empty where not needed)
-std::vector<Tensor> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, OptTensor saved,
-                                   int64_t act, bool need_x, bool need_w, bool need_b,
-                                   torch::ScalarType weight_type,
-                                   torch::ScalarType bias_type) {
-  TORCH_CHECK_VALUE(x.is_cuda(), "x must be on a GPU");
+// saved: z, or y of a relu; -> dx, dweight, dbias (undefined where not needed)
+std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor saved,
+                                     int64_t act, bool need_x, bool need_w, bool need_b,
+                                     torch::ScalarType bias_type) {
   const int dtype = linear_dtype(x, "x");
   const int64_t n = weight.size(0), k = weight.size(1);
-  check_device(dy, x, "dy");
-  check_device(weight, x, "weight");
-  TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type() &&
-                       weight.scalar_type() == x.scalar_type(),
-                   "dy and weight must be of x's type");
-  TORCH_CHECK_VALUE(x.size(-1) == k && dy.size(-1) == n && dy.numel() / n == x.numel() / k,
-                    "dy, x and weight do not fit together");
-  TORCH_CHECK_VALUE(act == blk::kNone || (saved.has_value() && saved->is_contiguous() &&
-                                          saved->numel() == dy.numel() &&
-                                          saved->scalar_type() == x.scalar_type()),
-                    "the forward pass's values are missing");
   const c10::DeviceGuard guard(x.device());
-  const Rows yr = rows_of(dy), xr = rows_of(x), wr = rows_of(weight);
+  const Rows yr = rows_of(dy), xr = rows_of(x);
   const int64_t rows = xr.rows;
-  Tensor dx = torch::empty(need_x ? x.sizes().vec() : std::vector<int64_t>{0}, x.options());
-  Tensor dw = torch::empty({need_w ? n : 0, k}, x.options().dtype(weight_type));
-  Tensor db = torch::empty({need_b ? n : 0}, x.options().dtype(bias_type));
+  Tensor dx, dw, db;
+  if (need_x) dx = torch::empty(x.sizes(), x.options());
+  if (need_w) dw = torch::empty({n, k}, weight.options());
+  if (need_b) db = torch::empty({n}, x.options().dtype(bias_type));
   if (!rows) {
-    dw.zero_();
-    db.zero_();
+    if (need_w) dw.zero_();
+    if (need_b) db.zero_();
     return {dx, dw, db};
   }
   const hipStream_t stream = stream_of(x);
@@ -435,13 +537,14 @@ std::vector<Tensor> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, OptTensor
   if (act || need_b) {
     blk::ActBwd b{};
     b.blocks = blk::act_bwd_blocks(rows, n);
-    Tensor partial = torch::empty({need_b ? b.blocks * n : 0},
-                                  x.options().dtype(torch::kFloat32));
+    Tensor partial;
+    if (need_b)
+      partial = torch::empty({b.blocks * n}, x.options().dtype(torch::kFloat32));
     b.dy = yr.t.data_ptr();
     if (act) {
       dz = torch::empty({rows, n}, x.options());
       dz_stride = n;
-      b.z = saved->data_ptr();
+      b.z = saved.data_ptr();
       b.dz = dz.data_ptr();
     }
     b.partial = need_b ? partial.data_ptr<float>() : nullptr;
@@ -455,6 +558,7 @@ std::vector<Tensor> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, OptTensor
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   if (need_x) {
+    const Rows wr = rows_of(weight.to(x.scalar_type()));
     blk::Product a{};
     a.p = dz.data_ptr();
     a.q = wr.t.data_ptr();
@@ -478,10 +582,54 @@ std::vector<Tensor> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, OptTensor
     a.r = rows;
     a.p_t = a.q_t = true;
     a.out = dw.data_ptr();
-    a.out_f32 = weight_type == torch::kFloat32;
+    a.out_f32 = weight.scalar_type() == torch::kFloat32;
     run_product(a, dtype, x);
   }
   return {dx, dw, db};
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  enum { kX = 1, kWeight = 2, kBias = 4, kResidual = 8 };
+
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, OptTensor bias,
+                        OptTensor residual, int64_t act) {
+    // a relu's sign can be read off its output where no residual covers it
+    const bool from_y = act == blk::kRelu && !residual.has_value();
+    const auto r = linear_act_fwd(x, weight, bias, residual, act,
+                                  act != blk::kNone && !from_y);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, weight, from_y ? r[0] : r[1]});
+    int64_t need = x.requires_grad() ? kX : 0;
+    if (weight.requires_grad()) need |= kWeight;
+    if (bias.has_value() && bias->requires_grad()) need |= kBias;
+    if (residual.has_value() && residual->requires_grad()) need |= kResidual;
+    ctx->saved_data["need"] = need;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["type"] = (int64_t)(bias.has_value() ? bias->scalar_type()
+                                                         : x.scalar_type());
+    return r[0];
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const Tensor dy = grads[0];
+    std::array<Tensor, 3> r;
+    if (dy.defined() && need & (kX | kWeight | kBias))
+      r = linear_act_bwd(dy, saved[0], saved[1], saved[2],
+                         ctx->saved_data["act"].toInt(), need & kX, need & kWeight,
+                         need & kBias,
+                         (torch::ScalarType)ctx->saved_data["type"].toInt());
+    return once({r[0], r[1], r[2], need & kResidual ? dy : Tensor(), Tensor()},
+                "linear_act");
+  }
+};
+
+Tensor linear_act(Tensor x, Tensor weight, OptTensor bias, OptTensor residual, int64_t act) {
+  const OptTensor leaf = x, w = weight;
+  if (wants_grad({&leaf, &w, &bias, &residual}))
+    return LinearAct::apply(x, weight, bias, residual, act);
+  return linear_act_fwd(x, weight, bias, residual, act, false)[0];
 }
 
 // ----------------------------------------------------------- gradient norm
@@ -500,8 +648,8 @@ void sort_spans(std::vector<Span>& v) {
   if (!std::is_sorted(v.begin(), v.end())) std::sort(v.begin(), v.end());
 }
 
-// -> norm, coefficient; scales into `outs`, or in place where that is `grads`
-std::vector<Tensor> clip_grad_norm(std::vector<Tensor> grads,
+// -> norm; scales into `outs`, or in place without them
+Tensor clip_grad_norm(std::vector<Tensor> grads,
                                    c10::optional<std::vector<Tensor>> outs,
                                    int64_t order, double max_norm, double eps,
                                    bool scale) {
@@ -554,6 +702,8 @@ std::vector<Tensor> clip_grad_norm(std::vector<Tensor> grads,
       written.push_back(span_of(out));
     }
     g[i].out_dtype = dtype_of(out, "an output");
+    // autograd notices a change of what it has saved by the version
+    if (scale && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     g[i].in = in.data_ptr();
     g[i].out = out.data_ptr();
   }
@@ -584,21 +734,19 @@ std::vector<Tensor> clip_grad_norm(std::vector<Tensor> grads,
     C10_HIP_KERNEL_LAUNCH_CHECK();
     for (auto& p : back) p.first.copy_(p.second);
   }
-  return {norm, coef};
+  return norm;
 }
 
 }  // namespace
 
 void register_block_ops(pybind11::module_& m) {
-  m.def("layer_norm_fwd", &layer_norm_fwd,
-        "layer norm of rows, behind an optional residual sum");
-  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward");
-  m.def("token_logprobs_fwd", &token_logprobs_fwd,
+  m.def("layer_norm", &layer_norm, "layer norm of rows");
+  m.def("add_layer_norm", &add_layer_norm,
+        "residual sum and layer norm of rows -> (y, sum)");
+  m.def("token_logprobs", &token_logprobs,
         "log probabilities of tokens, entropy and top alternatives");
-  m.def("token_logprobs_bwd", &token_logprobs_bwd, "token log probabilities backward");
-  m.def("linear_act_fwd", &linear_act_fwd,
+  m.def("linear_act", &linear_act,
         "linear layer with bias, activation and residual (MFMA)");
-  m.def("linear_act_bwd", &linear_act_bwd, "linear layer with epilogue, backward");
   m.def("clip_grad_norm", &clip_grad_norm,
         "norm of a list of tensors, and their scaling to a largest norm");
 }

@@ -15,7 +15,6 @@ width and type, the statistics are those of the sum as it is stored.
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 
@@ -30,33 +29,6 @@ def _eager(s, weight, bias, eps):
     if bias is not None:
         y = y + bias.to(s.dtype)
     return y.to(dtype)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps):
-        ops = hip_ext.require()
-        y, s, mean, rstd = ops.layer_norm_fwd(x, residual, weight, bias, eps, True)
-        ctx.save_for_backward(s, mean, rstd, weight)
-        ctx.set_materialize_grads(False)
-        ctx.param_type = next((p.dtype for p in (weight, bias) if p is not None), None)
-        if residual is None:
-            return y
-        return y, s
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        s, mean, rstd, weight = ctx.saved_tensors
-        need_x, need_r, need_w, need_b, _ = ctx.needs_input_grad
-        if dy is None:                       # only the stream was used
-            return ds if need_x else None, ds if need_r else None, None, None, None
-        ops = hip_ext.require()
-        dx, dw, db = ops.layer_norm_bwd(
-            dy.to(s.dtype), None if ds is None else ds.to(s.dtype), s, mean, rstd,
-            weight, need_w or need_b, ctx.param_type or s.dtype)
-        return (dx if need_x else None, dx if need_r else None,
-                dw if need_w else None, db if need_b else None, None)
 
 
 def _check(x, weight, bias, eps):
@@ -78,13 +50,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     x: (..., C) float32, bfloat16 or float16; weight, bias: (C,) in float32 or
     x's type (both in one), or None.  Returns x's shape and type.
     """
+    ext = hip_ext.maybe_ext(x)
+    if ext is not None:
+        return ext.layer_norm(x, weight, bias, eps)
     _check(x, weight, bias, eps)
-    if hip_ext.maybe_ext(x) is None:
-        return _eager(x, weight, bias, eps)
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNorm.apply(x, None, weight, bias, eps)
-    return hip_ext.require().layer_norm_fwd(x, None, weight, bias, eps, False)[0]
+    return _eager(x, weight, bias, eps)
 
 
 def add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5):
@@ -93,20 +63,17 @@ def add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5):
     residual has x's shape and type; s is stored in that type and normalised as
     stored.  Gradients of both outputs flow to both inputs.
     """
+    ext = hip_ext.maybe_ext(x)
+    if ext is not None:
+        return ext.add_layer_norm(x, residual, weight, bias, eps)
     _check(x, weight, bias, eps)
     if residual.shape != x.shape:
         raise ValueError(f'residual has shape {tuple(residual.shape)}, but x has '
                          f'{tuple(x.shape)}')
     if residual.dtype != x.dtype:
         raise TypeError(f'residual is {residual.dtype}, but x is {x.dtype}')
-    if hip_ext.maybe_ext(x) is None:
-        s = x + residual
-        return _eager(s, weight, bias, eps), s
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, residual, weight, bias)):
-        return _LayerNorm.apply(x, residual, weight, bias, eps)
-    return tuple(hip_ext.require().layer_norm_fwd(x, residual, weight, bias, eps,
-                                                  False)[:2])
+    s = x + residual
+    return _eager(s, weight, bias, eps), s
 
 
 class FusedLayerNorm(nn.LayerNorm):

@@ -13,40 +13,10 @@ On a GPU the kernels in `ops/hip/linear_act.hip` run; CPU tensors (and
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 
 ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
-
-
-class _LinearAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        ops = hip_ext.require()
-        w = weight.to(x.dtype)
-        # a relu's sign can be read off its output where no residual covers it
-        from_y = act == ACTIVATIONS['relu'] and residual is None
-        y, z = ops.linear_act_fwd(x, w, bias, residual, act, act != 0 and not from_y)
-        ctx.save_for_backward(x, w, None if act == 0 else y if from_y else z)
-        ctx.act = act
-        ctx.weight_type = weight.dtype
-        ctx.bias_type = weight.dtype if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, saved = ctx.saved_tensors
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        dx = dw = db = None
-        dy = dy.to(x.dtype)
-        if need_x or need_w or need_b:
-            dx, dw, db = hip_ext.require().linear_act_bwd(
-                dy, x, w, saved, ctx.act, need_x, need_w, need_b,
-                ctx.weight_type, ctx.bias_type)
-        return (dx if need_x else None, dw if need_w else None,
-                db if need_b else None, dy if need_r else None, None)
 
 
 def _eager(x, weight, bias, activation, residual):
@@ -76,6 +46,9 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
     if activation not in ACTIVATIONS:
         raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got '
                          f'{activation!r}')
+    ext = hip_ext.maybe_ext(x)
+    if ext is not None:
+        return ext.linear_act(x, weight, bias, residual, ACTIVATIONS[activation])
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f'x of shape {tuple(x.shape)} does not fit a weight of shape '
                          f'{tuple(weight.shape)}')
@@ -94,14 +67,7 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
                              f'{(*x.shape[:-1], weight.shape[0])}')
         if residual.dtype != x.dtype:
             raise TypeError(f'residual is {residual.dtype}, but x is {x.dtype}')
-    if hip_ext.maybe_ext(x) is None:
-        return _eager(x, weight, bias, activation, residual)
-    act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _LinearAct.apply(x, weight, bias, residual, act)
-    return hip_ext.require().linear_act_fwd(x, weight.to(x.dtype), bias, residual, act,
-                                            False)[0]
+    return _eager(x, weight, bias, activation, residual)
 
 
 class LinearAct(nn.Linear):

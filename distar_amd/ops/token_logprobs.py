@@ -14,7 +14,6 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 
@@ -26,29 +25,6 @@ class TokenLogProbs(NamedTuple):
     entropy: torch.Tensor                    # (...) float32
     top_logprobs: Optional[torch.Tensor]     # (..., k) float32, no gradient
     top_tokens: Optional[torch.Tensor]       # (..., k) int64
-
-
-class _TokenLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, mask, temperature, top_k, ignore_index):
-        ops = hip_ext.require()
-        logprob, entropy, row_max, row_logsum, top_lp, top_t = ops.token_logprobs_fwd(
-            logits, tokens, mask, temperature, top_k, ignore_index, True)
-        ctx.save_for_backward(logits, tokens, mask, entropy, row_max, row_logsum)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
-        ctx.mark_non_differentiable(top_lp, top_t)
-        ctx.set_materialize_grads(False)
-        return logprob, entropy, top_lp, top_t
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogprob, dentropy, _lp, _t):
-        ops = hip_ext.require()
-        logits, tokens, mask, entropy, row_max, row_logsum = ctx.saved_tensors
-        dlogits = ops.token_logprobs_bwd(logits, tokens, mask, entropy, row_max,
-                                         row_logsum, dlogprob, dentropy,
-                                         ctx.temperature, ctx.ignore_index)
-        return dlogits, None, None, None, None, None
 
 
 def _eager(logits, tokens, mask, temperature, top_k, ignore_index):
@@ -104,6 +80,10 @@ def token_logprobs(logits, tokens, mask=None, temperature=1.0, top_k=0,
     NaN or +inf among a row's possible logits makes that row's results NaN (and
     its alternatives -1).
     """
+    ext = hip_ext.maybe_ext(logits)
+    if ext is not None:
+        return TokenLogProbs(*ext.token_logprobs(logits, tokens, mask, temperature, top_k,
+                                                 ignore_index))
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError('logits need a last dimension of at least one element')
     if not logits.is_floating_point():
@@ -126,13 +106,5 @@ def token_logprobs(logits, tokens, mask=None, temperature=1.0, top_k=0,
         except RuntimeError:
             raise ValueError(f'mask of shape {tuple(mask.shape)} does not broadcast to '
                              f'logits of shape {tuple(logits.shape)}') from None
-    if hip_ext.maybe_ext(logits) is None:
-        got = _eager(logits, tokens, mask, temperature, top_k, ignore_index)
-    elif torch.is_grad_enabled() and logits.requires_grad:
-        got = _TokenLogProbs.apply(logits, tokens, mask, float(temperature), top_k,
-                                   ignore_index)
-    else:
-        r = hip_ext.require().token_logprobs_fwd(logits, tokens, mask, temperature,
-                                                 top_k, ignore_index, False)
-        got = r[0], r[1], r[4], r[5]
+    got = _eager(logits, tokens, mask, temperature, top_k, ignore_index)
     return TokenLogProbs(got[0], got[1], *(got[2:] if top_k else (None, None)))

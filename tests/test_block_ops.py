@@ -705,3 +705,21 @@ def test_block_step_in_graph_and_on_another_stream():
         for graph, out in graphs:
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_second_derivatives_are_refused_and_versions_kept(device):
+    if device == 'cuda':
+        x = torch.randn(4, 8, device=device, dtype=torch.bfloat16, requires_grad=True)
+        w = torch.randn(8, 8, device=device, dtype=torch.bfloat16, requires_grad=True)
+        tokens = torch.zeros(4, dtype=torch.long, device=device)
+        for y in (layer_norm(x, w[0]), linear_act(x, w, None, 'gelu'), token_logprobs(x, tokens)[0]):
+            g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+            with pytest.raises(RuntimeError):
+                g.float().sum().backward()
+    a = torch.randn(5, device=device, requires_grad=True)
+    b = torch.randn(5, device=device)
+    y = (a * b).sum()
+    clip_grad_norm([b], 0.1)
+    with pytest.raises(RuntimeError):
+        y.backward()
