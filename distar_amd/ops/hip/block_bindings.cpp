@@ -312,7 +312,8 @@ LogitRows check_logits(const Tensor& logits, const Tensor& tokens,
 }
 
 // -> logprob, entropy, top_logprobs, top_tokens (both of width 0 without top_k),
-//    stats (maximum, log of the sum; undefined if unasked)
+//    stats (maximum, log of the sum, entropy, token of each row; undefined if
+//    unasked)
 std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor mask,
                                        double temperature, int64_t top_k,
                                        int64_t ignore_index, bool stats) {
@@ -328,7 +329,7 @@ std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor
   Tensor logprob = torch::empty(tokens.sizes(), f32);
   Tensor entropy = torch::empty(tokens.sizes(), f32);
   Tensor kept, top_lp, top_t;
-  if (stats) kept = torch::empty({2, rows}, f32);
+  if (stats) kept = torch::empty({rows, 4}, f32);
   if (top_k) {
     std::vector<int64_t> shape = tokens.sizes().vec();
     shape.push_back(k);
@@ -342,8 +343,7 @@ std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor
     a.mask = mask.has_value() ? (const uint8_t*)r.mask.t.data_ptr() : nullptr;
     a.logprob = logprob.data_ptr<float>();
     a.entropy = entropy.data_ptr<float>();
-    a.row_max = stats ? kept.data_ptr<float>() : nullptr;
-    a.row_logsum = stats ? a.row_max + rows : nullptr;
+    a.stats = stats ? kept.data_ptr<float>() : nullptr;
     a.top_logprobs = k ? top_lp.data_ptr<float>() : nullptr;
     a.top_tokens = k ? top_t.data_ptr<int64_t>() : nullptr;
     a.rows = rows;
@@ -359,36 +359,30 @@ std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor
   return {logprob, entropy, top_lp, top_t, kept};
 }
 
-Tensor token_logprobs_bwd(Tensor logits, Tensor tokens, OptTensor mask,
-                          Tensor entropy, Tensor stats, OptTensor dlogprob,
-                          OptTensor dentropy, double temperature,
-                          int64_t ignore_index) {
+Tensor token_logprobs_bwd(const Tensor& logits, const OptTensor& mask,
+                          const Tensor& stats, OptTensor dlogprob, OptTensor dentropy,
+                          double temperature) {
   const c10::DeviceGuard guard(logits.device());
-  const LogitRows r = check_logits(logits, tokens, mask);
-  const int64_t rows = r.logits.rows;
-  for (OptTensor* t : {&dlogprob, &dentropy}) {
-    if (!t->has_value()) continue;
-    *t = (*t)->to(torch::kFloat32).contiguous();
-  }
+  const Rows l = rows_of(logits);
+  Rows m;
+  if (mask.has_value()) m = rows_of(mask->expand(logits.sizes()));
+  for (OptTensor* t : {&dlogprob, &dentropy})
+    if (t->has_value()) *t = (*t)->to(torch::kFloat32).contiguous();
   Tensor dlogits = torch::empty(logits.sizes(), logits.options());
-  if (rows) {
+  if (l.rows) {
     blk::LogProbsBwd a{};
-    a.logits = r.logits.t.data_ptr();
-    a.tokens = r.tokens.data_ptr<int64_t>();
-    a.mask = mask.has_value() ? (const uint8_t*)r.mask.t.data_ptr() : nullptr;
-    a.entropy = entropy.data_ptr<float>();
-    a.row_max = stats.data_ptr<float>();
-    a.row_logsum = a.row_max + rows;
+    a.logits = l.t.data_ptr();
+    a.mask = mask.has_value() ? (const uint8_t*)m.t.data_ptr() : nullptr;
+    a.stats = stats.data_ptr<float>();
     a.dlogprob = (const float*)ptr(dlogprob);
     a.dentropy = (const float*)ptr(dentropy);
     a.dlogits = dlogits.data_ptr();
-    a.rows = rows;
-    a.stride = r.logits.stride;
-    a.mask_stride = mask.has_value() ? r.mask.stride : 0;
-    a.ignore_index = ignore_index;
+    a.rows = l.rows;
+    a.stride = l.stride;
+    a.mask_stride = mask.has_value() ? m.stride : 0;
     a.width = (int)logits.size(-1);
     a.inv_temperature = (float)(1.0 / temperature);
-    blk::token_logprobs_bwd(a, r.dtype, stream_of(logits));
+    blk::token_logprobs_bwd(a, dtype_of(logits, "logits"), stream_of(logits));
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   return dlogits;
@@ -401,9 +395,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     const auto r = token_logprobs_fwd(logits, tokens, mask, temperature, top_k,
                                       ignore_index, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, tokens, none_or(mask), r[1], r[4]});
+    ctx->save_for_backward({logits, none_or(mask), r[4]});
     ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["ignore_index"] = ignore_index;
     if (!top_k) return {r[0], r[1]};
     ctx->mark_non_differentiable({r[2], r[3]});
     return {r[0], r[1], r[2], r[3]};
@@ -413,10 +406,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     const auto saved = ctx->get_saved_variables();
     Tensor d;
     if (grads[0].defined() || grads[1].defined())
-      d = token_logprobs_bwd(saved[0], saved[1], opt(saved[2]), saved[3], saved[4],
-                             opt(grads[0]), opt(grads[1]),
-                             ctx->saved_data["temperature"].toDouble(),
-                             ctx->saved_data["ignore_index"].toInt());
+      d = token_logprobs_bwd(saved[0], opt(saved[1]), saved[2], opt(grads[0]),
+                             opt(grads[1]), ctx->saved_data["temperature"].toDouble());
     return once({d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "token_logprobs");
   }
 };

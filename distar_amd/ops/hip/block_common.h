@@ -58,18 +58,45 @@ __device__ __forceinline__ void store_some(T* p, int n, const float (&v)[V]) {
 template <typename T>
 __device__ __forceinline__ float rounded(float v) { return (float)(T)v; }
 
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) v += __shfl_xor(v, o, 64);
+// The value of a lane in the other half of this lane's 2 D lanes, by a move
+// between registers: that lane is the one D away for 1 and 2, and the mirrored
+// one for 4 and 8, which does as well once the halves agree within themselves.
+template <int D>
+__device__ __forceinline__ int lane_across(int v) {
+  if constexpr (D == 1) return __builtin_amdgcn_update_dpp(v, v, 0xB1, 15, 15, true);
+  if constexpr (D == 2) return __builtin_amdgcn_update_dpp(v, v, 0x4E, 15, 15, true);
+  if constexpr (D == 4) return __builtin_amdgcn_update_dpp(v, v, 0x141, 15, 15, true);
+  return __builtin_amdgcn_update_dpp(v, v, 0x140, 15, 15, true);
+}
+
+// f over LANES neighbouring lanes, the same in all of them
+template <int LANES, typename F>
+__device__ __forceinline__ float lanes_all(float v, F f) {
+  if constexpr (LANES > 1) v = f(v, __int_as_float(lane_across<1>(__float_as_int(v))));
+  if constexpr (LANES > 2) v = f(v, __int_as_float(lane_across<2>(__float_as_int(v))));
+  if constexpr (LANES > 4) v = f(v, __int_as_float(lane_across<4>(__float_as_int(v))));
+  if constexpr (LANES > 8) v = f(v, __int_as_float(lane_across<8>(__float_as_int(v))));
+  if constexpr (LANES > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v),
+                                                    false, false);
+    v = f(__int_as_float(r[0]), __int_as_float(r[1]));
+  }
+  if constexpr (LANES > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v),
+                                                    false, false);
+    v = f(__int_as_float(r[0]), __int_as_float(r[1]));
+  }
   return v;
 }
 
 template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_all<LANES>(v, [](float a, float b) { return a + b; });
+}
+
+template <int LANES>
 __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  return lanes_all<LANES>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 }  // namespace blk

@@ -36,7 +36,7 @@ struct LogProbs {
   const int64_t *tokens;
   const uint8_t *mask;                        // or null; 1: allowed
   float *logprob, *entropy;
-  float *row_max, *row_logsum;                // or null
+  float *stats;                               // [rows][4] or null
   float *top_logprobs;                        // or null, [rows][top_k]
   int64_t *top_tokens;
   int64_t rows, stride, mask_stride, ignore_index;
@@ -45,12 +45,11 @@ struct LogProbs {
 };
 struct LogProbsBwd {
   const void *logits;
-  const int64_t *tokens;
   const uint8_t *mask;
-  const float *entropy, *row_max, *row_logsum;
+  const float *stats;                         // the forward pass's
   const float *dlogprob, *dentropy;           // or null
   void *dlogits;                              // contiguous
-  int64_t rows, stride, mask_stride, ignore_index;
+  int64_t rows, stride, mask_stride;
   int width;
   float inv_temperature;
 };
