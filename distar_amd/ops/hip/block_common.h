@@ -54,6 +54,46 @@ __device__ __forceinline__ void store_some(T* p, int n, const float (&v)[V]) {
   }
 }
 
+// The 16-byte run of a row that starts at c, without a branch: the last one,
+// where less than a run is left, moves back to end with the row, and one that
+// would start behind the row takes the same place. The elements that this adds
+// are another run's: they are loaded, but neither count nor are stored. A load's
+// address then needs no condition, so all loads of a row are under way at once;
+// behind branches they wait for each other. Rows narrower than a run (NARROW)
+// are taken element by element.
+template <typename T, bool NARROW = false>
+struct RowRun {
+  static constexpr int V = Width<T>::v;
+  int c, at, width;
+
+  __device__ __forceinline__ RowRun(int c_, int width_)
+      : c(c_), at(NARROW ? c_ : min(c_, width_ - Width<T>::v)), width(width_) {}
+
+  __device__ __forceinline__ bool any() const { return c < width; }
+  __device__ __forceinline__ bool whole() const {
+    return NARROW ? c + V <= width : at == c;
+  }
+  __device__ __forceinline__ bool counts(int i) const {
+    return NARROW ? c + i < width : at + i >= c;
+  }
+  // of a row of any type
+  template <typename E>
+  __device__ __forceinline__ void load(const E* row, float (&o)[V]) const {
+    if constexpr (NARROW) load_some<E, V>(row + at, width - at, o, 0.f);
+    else load_run<E, V>(row + at, o);
+  }
+  template <typename E>
+  __device__ __forceinline__ void store(E* row, const float (&v)[V]) const {
+    if (whole()) {
+      store_run<E, V>(row + at, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (counts(i)) row[at + i] = (E)v[i];
+    }
+  }
+};
+
 // what a store in T and a load of it give
 template <typename T>
 __device__ __forceinline__ float rounded(float v) { return (float)(T)v; }

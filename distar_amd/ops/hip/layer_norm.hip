@@ -41,67 +41,83 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   }
 }
 
-template <typename T, typename WT, int TPR, int NV>
+template <typename T, typename WT, int TPR, int NV, bool NARROW>
 __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads)
 void ln_fwd_kernel(LayerNormFwd a) {
   constexpr int V = Width<T>::v;
   constexpr int RPB = (TPR > kThreads ? TPR : kThreads) / TPR;
+  using Run = RowRun<T, NARROW>;
   __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x % TPR;
   const float inv = 1.f / (float)a.width;
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows;
        row0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = row0 + threadIdx.x / TPR;
-    const bool some = row < a.rows;
+    const int64_t mine = row0 + threadIdx.x / TPR;
+    const bool some = mine < a.rows;
+    const int64_t row = some ? mine : a.rows - 1;
     const T* x = (const T*)a.x + row * a.x_stride;
     const T* r = (const T*)a.residual + row * a.r_stride;
-    float v[NV][V];
+    float v[NV][V], q[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) Run((j * TPR + t) * V, a.width).load(x, v[j]);
+    if (a.residual) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) Run((j * TPR + t) * V, a.width).load(r, q[j]);
+    }
+    float w[NV][V], b[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const Run run((j * TPR + t) * V, a.width);
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[j][i] = 1.f, b[j][i] = 0.f;
+      if (a.weight) run.load((const WT*)a.weight, w[j]);
+      if (a.bias) run.load((const WT*)a.bias, b[j]);
+    }
+    if (a.residual) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = rounded<T>(v[j][i] + q[j][i]);
+        if (some)
+          Run((j * TPR + t) * V, a.width).store((T*)a.s + row * a.width, v[j]);
+      }
+    }
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + t) * V;
-      const int n = some ? a.width - c : 0;
-      if (n <= 0) {
+      const Run run((j * TPR + t) * V, a.width);
+      if (run.whole()) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = 0.f;
-        continue;
+        for (int i = 0; i < V; ++i) sum += v[j][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += run.counts(i) ? v[j][i] : 0.f;
       }
-      load_some<T, V>(x + c, n, v[j], 0.f);
-      if (a.residual) {
-        float q[V];
-        load_some<T, V>(r + c, n, q, 0.f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = rounded<T>(v[j][i] + q[i]);
-        store_some<T, V>((T*)a.s + row * a.width + c, n, v[j]);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += v[j][i];
     }
     const float mean = row_sum<TPR>(sum, lds) * inv;
     float sq = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      const Run run((j * TPR + t) * V, a.width);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = v[j][i] - mean;
-        if ((j * TPR + t) * V + i < a.width) sq += d * d;
+      for (int i = 0; i < V; ++i) v[j][i] -= mean;
+      if (run.whole()) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq += v[j][i] * v[j][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq += run.counts(i) ? v[j][i] * v[j][i] : 0.f;
       }
+    }
     const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, lds) * inv + a.eps);
+    if (!some) continue;                 // only rows that share a block
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + t) * V;
-      const int n = some ? a.width - c : 0;
-      if (n <= 0) continue;
-      float w[V], b[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = 1.f, b[i] = 0.f;
-      if (a.weight) load_some<WT, V>((const WT*)a.weight + c, n, w, 0.f);
-      if (a.bias) load_some<WT, V>((const WT*)a.bias + c, n, b, 0.f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = (v[j][i] - mean) * rstd * w[i] + b[i];
-      store_some<T, V>((T*)a.y + row * a.width + c, n, w);
+      for (int i = 0; i < V; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
+      Run((j * TPR + t) * V, a.width).store((T*)a.y + row * a.width, v[j]);
     }
-    if (a.mean && some && t == 0) {
+    if (a.mean && t == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
@@ -159,12 +175,13 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(LayerNormFwd a) {
   }
 }
 
-template <typename T, typename WT, int TPR, int NV>
+template <typename T, typename WT, int TPR, int NV, bool NARROW>
 __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads)
 void ln_bwd_kernel(LayerNormBwd a) {
   constexpr int V = Width<T>::v;
   constexpr int NT = TPR > kThreads ? TPR : kThreads;
   constexpr int RPB = NT / TPR;
+  using Run = RowRun<T, NARROW>;
   __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
   __shared__ float part[RPB > 1 ? NT * V : 1];
   const int t = threadIdx.x % TPR;
@@ -172,58 +189,55 @@ void ln_bwd_kernel(LayerNormBwd a) {
   float dw[NV][V] = {}, db[NV][V] = {};
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows;
        row0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = row0 + threadIdx.x / TPR;
-    const bool some = row < a.rows;
-    const float mean = some ? a.mean[row] : 0.f;
-    const float rstd = some ? a.rstd[row] : 0.f;
-    float g[NV][V], h[NV][V];
+    const int64_t mine = row0 + threadIdx.x / TPR;
+    const bool some = mine < a.rows;
+    const int64_t row = some ? mine : a.rows - 1;
+    float g[NV][V], h[NV][V], o[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const Run run((j * TPR + t) * V, a.width);
+      run.load((const T*)a.dy + row * a.dy_stride, g[j]);
+      run.load((const T*)a.s + row * a.s_stride, h[j]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[j][i] = 0.f;
+      if (a.ds) run.load((const T*)a.ds + row * a.ds_stride, o[j]);
+    }
+    const float mean = a.mean[row], rstd = a.rstd[row];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + t) * V;
-      const int n = some ? a.width - c : 0;
-      if (n <= 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[j][i] = h[j][i] = 0.f;
-        continue;
-      }
+      const Run run((j * TPR + t) * V, a.width);
       float w[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) w[i] = 1.f;
-      load_some<T, V>((const T*)a.dy + row * a.dy_stride + c, n, g[j], 0.f);
-      load_some<T, V>((const T*)a.s + row * a.s_stride + c, n, h[j], mean);
-      if (a.weight) load_some<WT, V>((const WT*)a.weight + c, n, w, 0.f);
+      if (a.weight) run.load((const WT*)a.weight, w);
+      const bool all = run.whole() && some;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         h[j][i] = (h[j][i] - mean) * rstd;
-        dw[j][i] += g[j][i] * h[j][i];
-        db[j][i] += g[j][i];
+        const float d = all || (some && run.counts(i)) ? g[j][i] : 0.f;
+        dw[j][i] += d * h[j][i];
+        db[j][i] += d;
         g[j][i] *= w[i];
-        s1 += g[j][i];
-        s2 += g[j][i] * h[j][i];
+        s1 += d * w[i];
+        s2 += d * w[i] * h[j][i];
       }
     }
     s1 = row_sum<TPR>(s1, lds) * inv;
     s2 = row_sum<TPR>(s2, lds) * inv;
+    if (!some) continue;                 // only rows that share a block
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + t) * V;
-      const int n = some ? a.width - c : 0;
-      if (n <= 0) continue;
-      float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = 0.f;
-      if (a.ds) load_some<T, V>((const T*)a.ds + row * a.ds_stride + c, n, o, 0.f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] += rstd * (g[j][i] - s1 - h[j][i] * s2);
-      store_some<T, V>((T*)a.dx + row * a.width + c, n, o);
+      for (int i = 0; i < V; ++i) o[j][i] += rstd * (g[j][i] - s1 - h[j][i] * s2);
+      Run((j * TPR + t) * V, a.width).store((T*)a.dx + row * a.width, o[j]);
     }
   }
   if (!a.partial) return;
   // rows that share a block: their sums are added in the order of the groups
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (j * TPR + t) * V;
+    const Run run((j * TPR + t) * V, a.width);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       float(&acc)[NV][V] = q ? db : dw;
@@ -237,9 +251,8 @@ void ln_bwd_kernel(LayerNormBwd a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[j][i] += part[(k * TPR + t) * V + i];
       }
-      if (threadIdx.x < TPR && c < a.width)
-        store_some<float, V>(a.partial + ((int64_t)blockIdx.x * 2 + q) * a.width + c,
-                             a.width - c, acc[j]);
+      if (threadIdx.x < TPR)
+        run.store(a.partial + ((int64_t)blockIdx.x * 2 + q) * a.width, acc[j]);
     }
   }
 }
@@ -342,22 +355,24 @@ void fwd(const LayerNormFwd& a, hipStream_t stream) {
   const int64_t rpb = rows_a_block(n);
   const int64_t need = (a.rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(need < (1 << 20) ? need : (1 << 20)));
-  if (n <= 8)
-    ln_fwd_kernel<T, WT, 8, 1><<<grid, 256, 0, stream>>>(a);
+  if (a.width < Width<T>::v)
+    ln_fwd_kernel<T, WT, 8, 1, true><<<grid, 256, 0, stream>>>(a);
+  else if (n <= 8)
+    ln_fwd_kernel<T, WT, 8, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 32)
-    ln_fwd_kernel<T, WT, 32, 1><<<grid, 256, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 32, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 64)
-    ln_fwd_kernel<T, WT, 64, 1><<<grid, 256, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 64, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 128)
-    ln_fwd_kernel<T, WT, 64, 2><<<grid, 256, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 64, 2, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 256)
-    ln_fwd_kernel<T, WT, 256, 1><<<grid, 256, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 256, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 512)
-    ln_fwd_kernel<T, WT, 256, 2><<<grid, 256, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 256, 2, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 1024)
-    ln_fwd_kernel<T, WT, 512, 2><<<grid, 512, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 512, 2, false><<<grid, 512, 0, stream>>>(a);
   else if (n <= kMaxRuns)
-    ln_fwd_kernel<T, WT, 1024, 2><<<grid, 1024, 0, stream>>>(a);
+    ln_fwd_kernel<T, WT, 1024, 2, false><<<grid, 1024, 0, stream>>>(a);
   else
     ln_fwd_wide_kernel<T, WT><<<grid, 1024, 0, stream>>>(a);
 }
@@ -366,22 +381,24 @@ template <typename T, typename WT>
 void bwd(const LayerNormBwd& a, hipStream_t stream) {
   const int n = runs<T>(a.width);
   const dim3 grid(a.blocks);
-  if (n <= 8)
-    ln_bwd_kernel<T, WT, 8, 1><<<grid, 256, 0, stream>>>(a);
+  if (a.width < Width<T>::v)
+    ln_bwd_kernel<T, WT, 8, 1, true><<<grid, 256, 0, stream>>>(a);
+  else if (n <= 8)
+    ln_bwd_kernel<T, WT, 8, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 32)
-    ln_bwd_kernel<T, WT, 32, 1><<<grid, 256, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 32, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 64)
-    ln_bwd_kernel<T, WT, 64, 1><<<grid, 256, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 64, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 128)
-    ln_bwd_kernel<T, WT, 64, 2><<<grid, 256, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 64, 2, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 256)
-    ln_bwd_kernel<T, WT, 256, 1><<<grid, 256, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 256, 1, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 512)
-    ln_bwd_kernel<T, WT, 256, 2><<<grid, 256, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 256, 2, false><<<grid, 256, 0, stream>>>(a);
   else if (n <= 1024)
-    ln_bwd_kernel<T, WT, 512, 2><<<grid, 512, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 512, 2, false><<<grid, 512, 0, stream>>>(a);
   else if (n <= kMaxRuns)
-    ln_bwd_kernel<T, WT, 1024, 2><<<grid, 1024, 0, stream>>>(a);
+    ln_bwd_kernel<T, WT, 1024, 2, false><<<grid, 1024, 0, stream>>>(a);
   else {
     const dim3 rows((unsigned)(a.rows < 65536 ? a.rows : 65536));
     ln_bwd_wide_kernel<T, WT><<<rows, 1024, 0, stream>>>(a);

@@ -1,26 +1,23 @@
 // Log probabilities of given tokens, the entropy of their distributions and
 // the likeliest alternatives, from one reading of the logits.
 //
-//   x_j = (l_j - m) / T over the allowed places, m = max l
-//   S = sum e^x,  U = sum x e^x
-//   logprob = x_t - log S       H = log S - U / S
+//   y_j = (l_j - m) / (T ln 2) over the allowed places, m = max l
+//   S = sum 2^y,  U = sum y 2^y
+//   logprob = ln 2 (y_t - log2 S)       H = ln 2 (log2 S - U / S)
 //   dl_j = (g_lp (d_tj - p_j) - g_H p_j (log p_j + H)) / T
 //
-// A place counts as having no probability where the mask is 0, whatever the
-// logit there holds, and where the logit is -inf. S and U are 32-bit sums.
-// Alternatives are ranked by the logits themselves, equal ones by their index,
-// so the temperature's rounding cannot reorder them.
-//
-// Forward, a row up to 32768 wide is read once and stays in the registers of
-// 8 to 1024 threads, which take its maximum, then the sums, then look for the
-// alternatives in it. A wider one runs through 1024 threads, each with a maximum
-// of its own that its sums follow, and is read again for alternatives.
+// Forward, a thread runs through its part of the row with a maximum of its own
+// that its sums follow, four 16-byte runs at a time with the next four under way;
+// the threads' maxima and sums are joined at the end, so a row is read once and
+// waits once. 64, 256 or 1024 threads take a row. Narrow rows without alternatives
+// lie in the registers of 8 or 16 threads instead.
 //
 // The k alternatives: of 64 maxima over disjoint parts of the row (one of each
 // lane) the k-th largest is a bound that at least k elements reach, and few more
-// do. Those that reach it go to a list in LDS, where each counts how many come
-// before it; the first k write themselves out. Only a row with very many equal
-// logits overflows the list: it is searched k times instead.
+// do. Only the few threads whose maximum reaches it read their part again; what
+// reaches it goes to a list in LDS, where each counts how many come before it, and
+// the first k write themselves out. Only a row with very many equal logits
+// overflows the list: it is searched k times instead.
 //
 // Backward, the gradient's memory is cut into aligned runs of 16 bytes whatever
 // the rows' width, and a run that holds the end of a row takes a slower way.
@@ -32,36 +29,41 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float exp_(float x) {
-  return __builtin_amdgcn_exp2f(x * kLog2e);
+__device__ __forceinline__ float exp2_(float y) {
+  return __builtin_amdgcn_exp2f(y);
 }
 
-// maximum, S and U of a part of a row
+__device__ __forceinline__ float log2_(float s) {
+  return __builtin_amdgcn_logf(s);
+}
+
+template <typename T>
+using Run = T __attribute__((ext_vector_type(Width<T>::v)));
+
+// maximum, S and U of a part of a row; S is NaN if that holds a NaN, or +inf
+// (from inf - inf)
 struct Stat {
   float m, s, u;
 };
-
-__device__ __forceinline__ Stat join(Stat a, Stat b, float inv_t) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  if (r.m == -kInf) return {-kInf, a.s + b.s, 0.f};   // S is 0, or NaN to keep
-  const float da = a.m == -kInf ? 0.f : (a.m - r.m) * inv_t;
-  const float db = b.m == -kInf ? 0.f : (b.m - r.m) * inv_t;
-  const float ea = exp_(da), eb = exp_(db);
-  r.s = a.s * ea + b.s * eb;
-  r.u = (a.u + da * a.s) * ea + (b.u + db * b.s) * eb;
-  return r;
-}
 
 __device__ __forceinline__ bool before(float v, int i, float w, int j) {
   return v > w || (v == w && i < j);
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_masked(const T* l, const uint8_t* mask,
-                                            int n, float (&v)[V]) {
-  load_some<T, V>(l, n, v, -kInf);
+// n elements of a row (at least one); -inf behind them and where the mask is 0
+template <typename T>
+__device__ __forceinline__ Run<T> load_masked(const T* l, const uint8_t* mask,
+                                              int n) {
+  constexpr int V = Width<T>::v;
+  Run<T> v;
+  if (n >= V) {
+    __builtin_memcpy(&v, l, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < n ? l[i] : (T)-kInf;
+  }
   if (mask) {
     uint8_t q[V];
     if (n >= V) {
@@ -71,8 +73,9 @@ __device__ __forceinline__ void load_masked(const T* l, const uint8_t* mask,
       for (int i = 0; i < V; ++i) q[i] = i < n ? mask[i] : 0;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = q[i] ? v[i] : -kInf;
+    for (int i = 0; i < V; ++i) v[i] = q[i] ? v[i] : (T)-kInf;
   }
+  return v;
 }
 
 constexpr int kList = 1024;         // alternatives' candidates of a block
@@ -105,236 +108,342 @@ __device__ __forceinline__ void row_sync() {
   }
 }
 
-// A row of at most TPR * V * NV elements in registers (NV > 0), or one of any
-// width that is loaded again each time (NV = 0).
-template <typename T, int TPR, int NV>
+// What a row's first thread leaves: its results but for the alternatives, and
+// what the backward pass needs. `given` is the token's logit, -inf if masked.
+__device__ __forceinline__ void leave(const LogProbs& a, int64_t row, Stat st,
+                                      float given, float scale) {
+  const int64_t token = a.tokens[row];
+  const bool ignored = token == a.ignore_index;
+  const bool inside = token >= 0 && token < a.width;
+  const bool empty = st.m == -kInf && st.s == 0.f;
+  const bool bad = st.s != st.s;
+  const float nan = __builtin_nanf("");
+  const float log2sum = log2_(st.s);
+  const float h = bad ? nan : empty ? 0.f : (log2sum - st.u / st.s) * kLn2;
+  a.logprob[row] = ignored ? 0.f
+                 : !inside || bad ? nan
+                 : given == -kInf ? -kInf
+                 : ((given - st.m) * scale - log2sum) * kLn2;
+  a.entropy[row] = h;
+  if (a.stats) {
+    const float4 keep = {bad ? nan : st.m, log2sum, h,
+                         __int_as_float(ignored ? -1 : inside ? (int)token : -2)};
+    *(float4*)(a.stats + row * 4) = keep;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float given_logit(const LogProbs& a, int64_t row) {
+  const int64_t token = a.tokens[row];
+  if (token < 0 || token >= a.width) return -kInf;
+  if (a.mask && !a.mask[row * a.mask_stride + token]) return -kInf;
+  return (float)((const T*)a.logits)[row * a.stride + token];
+}
+
+// Rows of at most TPR * V * NV elements, without alternatives.
+template <typename T, int TPR, int NV, bool NARROW>
+__global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
+  constexpr int V = Width<T>::v;
+  constexpr int RPB = 256 / TPR;
+  const int t = threadIdx.x % TPR;
+  const float scale = a.inv_temperature * kLog2e;
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows;
+       row0 += (int64_t)gridDim.x * RPB) {
+    const int64_t mine = row0 + threadIdx.x / TPR;
+    const int64_t row = mine < a.rows ? mine : a.rows - 1;
+    const T* l = (const T*)a.logits + row * a.stride;
+    const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    const float given = t == 0 ? given_logit<T>(a, row) : 0.f;
+    Run<T> v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const RowRun<T, NARROW> run((j * TPR + t) * V, a.width);
+      if constexpr (NARROW) {
+        v[j] = (Run<T>)(T)-kInf;
+        if (run.any()) v[j] = load_masked<T>(l + run.c, mask ? mask + run.c : nullptr,
+                                             a.width - run.c);
+      } else {
+        __builtin_memcpy(&v[j], l + run.at, 16);
+      }
+    }
+    if constexpr (!NARROW) {
+      if (mask) {
+        uint8_t q[NV][V];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          __builtin_memcpy(q[j], mask + RowRun<T>((j * TPR + t) * V, a.width).at, V);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[j][i] = q[j][i] ? v[j][i] : (T)-kInf;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const RowRun<T> run((j * TPR + t) * V, a.width);
+        if (run.whole()) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = run.counts(i) ? v[j][i] : (T)-kInf;
+      }
+    }
+    Stat st = {-kInf, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) st.m = fmaxf(st.m, (float)v[j][i]);
+    st.m = lanes_max<TPR>(st.m);
+    const float m = st.m == -kInf ? 0.f : st.m;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (NV > 1 && j * TPR * V >= a.width) break;    // the same for all
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float y = ((float)v[j][i] - m) * scale, e = exp2_(y);
+        st.s += e;
+        st.u += e * fmaxf(y, -1e30f);       // e is 0 there
+      }
+    }
+    st.s = lanes_sum<TPR>(st.s);
+    st.u = lanes_sum<TPR>(st.u);
+    if (t == 0 && mine < a.rows) leave(a, row, st, given, scale);
+  }
+}
+
+constexpr int kBatch = 4;           // runs of a thread under way together
+
+// A thread's runs of a row, TPR runs apart, a batch at a time.
+template <typename T, int TPR>
+struct Batch {
+  static constexpr int V = Width<T>::v;
+  Run<T> v[kBatch];
+  uint64_t q[kBatch];
+
+  __device__ __forceinline__ void load(const T* l, const uint8_t* mask, int c0,
+                                       int width) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      __builtin_memcpy(&v[j], l + RowRun<T>(c0 + j * TPR * V, width).at, 16);
+    if (mask) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        __builtin_memcpy(&q[j], mask + RowRun<T>(c0 + j * TPR * V, width).at, V);
+    }
+  }
+
+  // -inf in the places that the mask or the row's end take away
+  __device__ __forceinline__ void limit(bool masked, int c0, int width) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (masked) {
+        uint8_t keep[V];
+        __builtin_memcpy(keep, &q[j], V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = keep[i] ? v[j][i] : (T)-kInf;
+      }
+      const RowRun<T> run(c0 + j * TPR * V, width);
+      if (!run.whole()) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = run.counts(i) ? v[j][i] : (T)-kInf;
+      }
+    }
+  }
+};
+
+template <typename T, int TPR>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256)
 void logprobs_kernel(LogProbs a) {
   constexpr int V = Width<T>::v;
   constexpr int RPB = TPR > 64 ? 1 : 256 / TPR;
-  constexpr int R = NV ? NV : 1;
+  constexpr int W = Shared<TPR>::waves;
+  constexpr int kStep = TPR * V * kBatch;
   __shared__ Shared<TPR> sh;
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 63;
   const int wave = TPR > 64 ? threadIdx.x >> 6 : 0;
   const int slot = TPR > 64 ? 0 : threadIdx.x >> 6;     // the wave's list
-  const float inv_t = a.inv_temperature;
+  const float scale = a.inv_temperature * kLog2e;
+  const int width = a.width;
+  const bool narrow = width < V;
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows;
        row0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = row0 + threadIdx.x / TPR;
-    const int width = row < a.rows ? a.width : 0;
-    const int64_t at = row < a.rows ? row : 0;
-    const T* l = (const T*)a.logits + at * a.stride;
-    const uint8_t* mask = a.mask ? a.mask + at * a.mask_stride : nullptr;
-    // the given token's logit, asked for before the row
-    const int64_t token = a.tokens[at];
-    const bool inside = token >= 0 && token < a.width;
-    const float given = inside && (!mask || mask[token]) ? (float)l[token] : -kInf;
+    const int64_t mine = row0 + threadIdx.x / TPR;
+    const bool some = mine < a.rows;
+    const int64_t row = some ? mine : a.rows - 1;
+    const T* l = (const T*)a.logits + row * a.stride;
+    const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
+    const float given = t == 0 ? given_logit<T>(a, row) : 0.f;
 
-    float v[R][V];
-    float most = -kInf;                 // this thread's maximum
     Stat st = {-kInf, 0.f, 0.f};
-    if constexpr (NV > 0) {
+    auto add = [&](const Run<T>& v, float m) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = (j * TPR + t) * V;
-        if (c < width) {
-          load_masked<T, V>(l + c, mask ? mask + c : nullptr, width - c, v[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[j][i] = -kInf;
-        }
+      for (int i = 0; i < V; ++i) {
+        const float y = ((float)v[i] - m) * scale, e = exp2_(y);
+        st.s += e;
+        st.u += e * fmaxf(y, -1e30f);       // e is 0 there
       }
+    };
+    // the sums go over to a larger maximum; returns what to subtract
+    auto raise = [&](float most) {
+      const float m = fmaxf(st.m, most);
+      const float by = m == -kInf ? 0.f : m;
+      const float d = fmaxf((st.m - by) * scale, -1e30f), f = exp2_(d);
+      st.u = (st.u + d * st.s) * f;
+      st.s *= f;
+      st.m = m;
+      return by;
+    };
+    if (narrow) {
+      if (t == 0) {
+        const Run<T> v = load_masked<T>(l, mask, width);
+        float most = -kInf;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) most = fmaxf(most, v[j][i]);
-      st.m = lanes_max<TPR < 64 ? TPR : 64>(most);
-      if constexpr (TPR > 64) {
-        if (lane == 0) sh.most[wave] = st.m;
-        sh.lane_most[wave][lane] = most;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < Shared<TPR>::waves; ++w) st.m = fmaxf(st.m, sh.most[w]);
-      }
-      const float m = st.m == -kInf ? 0.f : st.m;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (NV > 1 && j * TPR * V >= a.width) break;    // the same for all
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float x = (v[j][i] - m) * inv_t, e = exp_(x);
-          st.s += e;
-          st.u += e * fmaxf(x, -1e30f);       // e is 0 there
-        }
-      }
-      st.s = lanes_sum<TPR < 64 ? TPR : 64>(st.s);
-      st.u = lanes_sum<TPR < 64 ? TPR : 64>(st.u);
-      if constexpr (TPR > 64) {
-        if (lane == 0) sh.stat[wave] = st;
-        __syncthreads();
-        st.s = st.u = 0.f;
-#pragma unroll
-        for (int w = 0; w < Shared<TPR>::waves; ++w)
-          st.s += sh.stat[w].s, st.u += sh.stat[w].u;
+        for (int i = 0; i < V; ++i) most = fmaxf(most, (float)v[i]);
+        add(v, raise(most));
       }
     } else {
-      for (int c = t * V; c < width; c += TPR * V) {
-        load_masked<T, V>(l + c, mask ? mask + c : nullptr, width - c, v[0]);
-        Stat q = {v[0][0], 0.f, 0.f};
+      Batch<T, TPR> now, next;
+      now.load(l, mask, t * V, width);
+      for (int c = 0; c < width; c += kStep) {
+        if (c + kStep < width) next.load(l, mask, c + kStep + t * V, width);
+        now.limit(mask, c + t * V, width);
+        float most = -kInf;
 #pragma unroll
-        for (int i = 1; i < V; ++i) q.m = fmaxf(q.m, v[0][i]);
-        const float m = q.m == -kInf ? 0.f : q.m;
+        for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float x = (v[0][i] - m) * inv_t, e = exp_(x);
-          q.s += e;
-          q.u += e * fmaxf(x, -1e30f);
+          for (int i = 0; i < V; ++i) most = fmaxf(most, (float)now.v[j][i]);
+        const float m = raise(most);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (c + j * TPR * V >= width) break;          // the same for all
+          add(now.v[j], m);
         }
-        st = join(st, q, inv_t);
+        now = next;
       }
-      most = st.m;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1)
-        st = join(st, {__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64),
-                       __shfl_xor(st.u, o, 64)}, inv_t);
-      if (lane == 0) sh.stat[wave] = st;
+    }
+    const float most = st.m;              // this thread's maximum
+    st.m = lanes_max<64>(most);
+    if constexpr (TPR > 64) {
+      if (lane == 0) sh.most[wave] = st.m;
       sh.lane_most[wave][lane] = most;
       __syncthreads();
-      st = sh.stat[0];
-      for (int w = 1; w < Shared<TPR>::waves; ++w) st = join(st, sh.stat[w], inv_t);
+#pragma unroll
+      for (int w = 0; w < W; ++w) st.m = fmaxf(st.m, sh.most[w]);
     }
-    const bool empty = st.m == -kInf && st.s == 0.f;
-    // a NaN, or an infinite logit, leaves no distribution
-    const bool bad = !empty && !(st.s > 0.f && st.s < kInf && st.m < kInf);
-    const float nan = __builtin_nanf("");
-    const float logsum = bad ? nan : __logf(st.s);
-    if (t == 0 && width) {
-      const bool ignored = token == a.ignore_index;
-      const float h = bad ? nan : empty ? 0.f : logsum - st.u / st.s;
-      float lp;
-      if (ignored) lp = 0.f;
-      else if (!inside || bad) lp = nan;
-      else if (given == -kInf) lp = -kInf;
-      else lp = (given - st.m) * inv_t - logsum;
-      a.logprob[row] = lp;
-      a.entropy[row] = h;
-      if (a.stats) {
-        const float4 keep = {bad ? nan : st.m, logsum, h,
-                             __int_as_float(ignored ? -1 : inside ? (int)token : -2)};
-        *(float4*)(a.stats + row * 4) = keep;
-      }
+    {
+      const float by = st.m == -kInf ? 0.f : st.m;
+      const float d = fmaxf((most - by) * scale, -1e30f), f = exp2_(d);
+      st.u = lanes_sum<64>((st.u + d * st.s) * f);
+      st.s = lanes_sum<64>(st.s * f);
     }
+    if constexpr (TPR > 64) {
+      if (lane == 0) sh.stat[wave] = st;
+      __syncthreads();
+      st.s = st.u = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) st.s += sh.stat[w].s, st.u += sh.stat[w].u;
+    }
+    if (t == 0 && some) leave(a, row, st, given, scale);
     if (!a.top_k) {
       if constexpr (TPR > 64) __syncthreads();     // sh is used by the next row
       continue;
     }
 
-    if constexpr (TPR >= 64) {
-      const int K = a.top_k;
-      float* out_lp = a.top_logprobs + row * K;
-      int64_t* out_t = a.top_tokens + row * K;
-      const bool none = bad || empty;
-      auto each = [&](auto f) {
-        if constexpr (NV > 0) {
+    const bool bad = st.s != st.s;
+    const bool none = bad || st.m == -kInf || !some;
+    const float log2sum = log2_(st.s);
+    const int K = a.top_k;
+    float* out_lp = a.top_logprobs + row * K;
+    int64_t* out_t = a.top_tokens + row * K;
+    // this thread's part of the row once more
+    auto each = [&](auto f) {
+      for (int c = t * V; c < width; c += TPR * V) {
+        const Run<T> v = load_masked<T>(l + c, mask ? mask + c : nullptr, width - c);
 #pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) f(v[j][i], (j * TPR + t) * V + i);
-        } else {
-          for (int c = t * V; c < width; c += TPR * V) {
-            load_masked<T, V>(l + c, mask ? mask + c : nullptr, width - c, v[0]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f(v[0][i], c + i);
+        for (int i = 0; i < V; ++i) f((float)v[i], c + i);
+      }
+    };
+    // the K-th largest of 64 lanes' maxima
+    float bound = most;
+    if (TPR == 64 || wave == 0) {
+      float g = most;
+      if constexpr (TPR > 64)
+        for (int w = 1; w < W; ++w) g = fmaxf(g, sh.lane_most[w][lane]);
+      for (int k = 0; k < K; ++k) {
+        bound = lanes_max<64>(g);
+        const uint64_t who = __ballot(g == bound);
+        if (who && lane == __ffsll((unsigned long long)who) - 1) g = -kInf;
+      }
+      if (lane == 0) {
+        sh.count[slot] = 0;
+        sh.bound = bound;
+      }
+    }
+    row_sync<TPR>();
+    if constexpr (TPR > 64) bound = sh.bound;
+    const int base = slot * Shared<TPR>::list;
+    if (!none && most >= bound)
+      each([&](float x, int c) {
+        if (x >= bound && x > -kInf) {
+          const int n = atomicAdd(&sh.count[slot], 1);
+          if (n < Shared<TPR>::list) {
+            sh.list_v[base + n] = x;
+            sh.list_i[base + n] = c;
           }
         }
-      };
-      // the K-th largest of 64 lanes' maxima
-      float bound = most;
-      if (TPR == 64 || wave == 0) {
-        float g = most;
-        if constexpr (TPR > 64)
-          for (int w = 1; w < Shared<TPR>::waves; ++w)
-            g = fmaxf(g, sh.lane_most[w][lane]);
-        for (int k = 0; k < K; ++k) {
-          bound = lanes_max<64>(g);
-          const uint64_t who = __ballot(g == bound);
-          if (who && lane == __ffsll((unsigned long long)who) - 1) g = -kInf;
-        }
-        if (lane == 0) {
-          sh.count[slot] = 0;
-          sh.bound = bound;
+      });
+    row_sync<TPR>();
+    const int n = none ? 0 : sh.count[slot];
+    if (n <= Shared<TPR>::list) {
+      for (int q = t; q < n; q += TPR) {
+        const float x = sh.list_v[base + q];
+        const int c = sh.list_i[base + q];
+        int rank = 0;
+        for (int o = 0; o < n; ++o)
+          rank += before(sh.list_v[base + o], sh.list_i[base + o], x, c);
+        if (rank < K) {
+          out_lp[rank] = ((x - st.m) * scale - log2sum) * kLn2;
+          out_t[rank] = c;
         }
       }
-      row_sync<TPR>();
-      if constexpr (TPR > 64) bound = sh.bound;
-      const int base = slot * Shared<TPR>::list;
-      if (!none && most >= bound)
+      if (some)
+        for (int k = n + t; k < K; k += TPR) {
+          out_lp[k] = bad ? __builtin_nanf("") : -kInf;
+          out_t[k] = -1;
+        }
+    } else {
+      // each the best behind the one before it; the list held more than K
+      float last_v = kInf;
+      int last_i = -1;
+      for (int k = 0; k < K; ++k) {
+        float bv = -kInf;
+        int bi = INT32_MAX;
         each([&](float x, int c) {
-          if (x >= bound && x > -kInf) {
-            const int n = atomicAdd(&sh.count[slot], 1);
-            if (n < Shared<TPR>::list) {
-              sh.list_v[base + n] = x;
-              sh.list_i[base + n] = c;
-            }
+          if (x > -kInf && before(last_v, last_i, x, c) && before(x, c, bv, bi)) {
+            bv = x;
+            bi = c;
           }
         });
-      row_sync<TPR>();
-      const int n = none ? 0 : sh.count[slot];
-      if (n <= Shared<TPR>::list) {
-        for (int q = t; q < n; q += TPR) {
-          const float x = sh.list_v[base + q];
-          const int c = sh.list_i[base + q];
-          int rank = 0;
-          for (int o = 0; o < n; ++o)
-            rank += before(sh.list_v[base + o], sh.list_i[base + o], x, c);
-          if (rank < K) {
-            out_lp[rank] = (x - st.m) * inv_t - logsum;
-            out_t[rank] = c;
-          }
-        }
-        if (width)
-          for (int k = n + t; k < K; k += TPR) {
-            out_lp[k] = bad ? nan : -kInf;
-            out_t[k] = -1;
-          }
-      } else {
-        // each the best behind the one before it
-        float last_v = kInf;
-        int last_i = -1;
-        for (int k = 0; k < K; ++k) {
-          float bv = -kInf;
-          int bi = INT32_MAX;
-          each([&](float x, int c) {
-            if (x > -kInf && before(last_v, last_i, x, c) && before(x, c, bv, bi)) {
-              bv = x;
-              bi = c;
-            }
-          });
 #pragma unroll
-          for (int o = 1; o < 64; o <<= 1) {
-            const float ov = __shfl_xor(bv, o, 64);
-            const int oi = __shfl_xor(bi, o, 64);
-            if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
-          }
-          if constexpr (TPR > 64) {
-            __syncthreads();
-            if (lane == 0) sh.best_v[wave] = bv, sh.best_i[wave] = bi;
-            __syncthreads();
-            bv = sh.best_v[0], bi = sh.best_i[0];
-            for (int w = 1; w < Shared<TPR>::waves; ++w)
-              if (before(sh.best_v[w], sh.best_i[w], bv, bi))
-                bv = sh.best_v[w], bi = sh.best_i[w];
-          }
-          // the list held more than K, so there is one
-          if (t == 0) {
-            out_lp[k] = (bv - st.m) * inv_t - logsum;
-            out_t[k] = bi;
-          }
-          last_v = bv, last_i = bi;
+        for (int o = 1; o < 64; o <<= 1) {
+          const float ov = __shfl_xor(bv, o, 64);
+          const int oi = __shfl_xor(bi, o, 64);
+          if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
         }
+        if constexpr (TPR > 64) {
+          __syncthreads();
+          if (lane == 0) sh.best_v[wave] = bv, sh.best_i[wave] = bi;
+          __syncthreads();
+          bv = sh.best_v[0], bi = sh.best_i[0];
+          for (int w = 1; w < W; ++w)
+            if (before(sh.best_v[w], sh.best_i[w], bv, bi))
+              bv = sh.best_v[w], bi = sh.best_i[w];
+        }
+        if (t == 0) {
+          out_lp[k] = ((bv - st.m) * scale - log2sum) * kLn2;
+          out_t[k] = bi;
+        }
+        last_v = bv, last_i = bi;
       }
-      row_sync<TPR>();
     }
+    row_sync<TPR>();
   }
 }
 
@@ -354,30 +463,28 @@ __device__ __forceinline__ uint32_t over(uint32_t n, Divide d) {
 }
 
 struct RowGrad {
-  float m, logsum, h, glp, gh;
+  float m, log2sum, h, glp, gh;
   int token;
-  bool empty;
 };
 
 __device__ __forceinline__ RowGrad row_grad(const LogProbsBwd& a, int64_t row) {
   const float4 s = *(const float4*)(a.stats + row * 4);
   RowGrad r;
-  r.m = s.x, r.logsum = s.y, r.h = s.z;
+  r.m = s.x, r.log2sum = s.y, r.h = s.z;
   r.token = __float_as_int(s.w);
   r.glp = a.dlogprob && r.token != -1 ? a.dlogprob[row] : 0.f;
   r.gh = a.dentropy ? a.dentropy[row] : 0.f;
-  r.empty = r.m == -kInf;
   return r;
 }
 
 __device__ __forceinline__ float logit_grad(const RowGrad& r, float l, int c,
-                                            float inv_t) {
-  const float lp = (l - r.m) * inv_t - r.logsum;
-  const float p = exp_(lp);
-  float d = -p * (r.glp + r.gh * (fmaxf(lp, -1e30f) + r.h));
-  d = lp != lp ? lp : d;
+                                            float scale, float inv_t) {
+  const float y = (l - r.m) * scale - r.log2sum;
+  const float p = exp2_(y);
+  float d = -p * (r.glp + r.gh * (fmaxf(y, -1e30f) * kLn2 + r.h));
+  d = y != y ? y : d;
   d += c == r.token ? r.glp : 0.f;
-  return r.empty ? 0.f : d * inv_t;
+  return r.m == -kInf ? 0.f : d * inv_t;      // a row without any token
 }
 
 constexpr int kBwdRuns = 4;           // runs a thread takes
@@ -386,67 +493,114 @@ template <typename T>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(LogProbsBwd a,
                                                            Divide by_width) {
   constexpr int V = Width<T>::v;
-  const float inv_t = a.inv_temperature;
-  const int64_t total = a.rows * a.width;
+  const float inv_t = a.inv_temperature, scale = inv_t * kLog2e;
+  const int width = a.width;
+  const int64_t total = a.rows * width;
   const int64_t base = (int64_t)blockIdx.x * (256 * V * kBwdRuns);
-  const int64_t row_b = base / a.width;
-  const uint32_t off_b = (uint32_t)(base - row_b * a.width);
+  const int64_t row_b = base / width;
+  const uint32_t off_b = (uint32_t)(base - row_b * width);
 #pragma unroll
   for (int k = 0; k < kBwdRuns; ++k) {
     const uint32_t o = (k * 256 + threadIdx.x) * V;
-    if (base + o >= total) break;
+    const int64_t left = total - (base + o);
+    if (left <= 0) break;
+    const int n = left < V ? (int)left : V;
     const uint32_t q = over(off_b + o, by_width);
-    int64_t row = row_b + q;
-    int c = (int)(off_b + o - q * (uint32_t)a.width);
+    const int64_t row = row_b + q;
+    const int c = (int)(off_b + o - q * (uint32_t)width);
     T* out = (T*)a.dlogits + base + o;
-    float d[V];
-    RowGrad r = row_grad(a, row);
-    if (c + V <= a.width) {
-      load_run<T, V>((const T*)a.logits + row * a.stride + c, d);
-      uint8_t allowed[V];
-      if (a.mask) __builtin_memcpy(allowed, a.mask + row * a.mask_stride + c, V);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[i] = logit_grad(r, d[i], c + i, inv_t);
-        if (a.mask && !allowed[i]) d[i] = 0.f;
+    if (width < V) {                  // many rows in a run
+      int64_t at = row;
+      int col = c;
+      for (int i = 0; i < n; ++i) {
+        const float x = logit_grad(row_grad(a, at),
+                                   (float)((const T*)a.logits)[at * a.stride + col],
+                                   col, scale, inv_t);
+        out[i] = a.mask && !a.mask[at * a.mask_stride + col] ? (T)0.f : (T)x;
+        if (++col == width) col = 0, ++at;
       }
+      continue;
+    }
+    // the run's first elements belong to this row, others to the next
+    const int here = width - c;
+    const T* l = (const T*)a.logits + row * a.stride + c;
+    const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride + c : nullptr;
+    float d[V];
+    uint8_t allowed[V];
+    if (n == V && (here >= V || a.stride == width)) {
+      load_run<T, V>(l, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        d[i] = i < n ? (float)l[i < here ? i : a.stride - width + i] : 0.f;
+    }
+    if (mask) {
+      if (n == V && (here >= V || a.mask_stride == width)) {
+        __builtin_memcpy(allowed, mask, V);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          allowed[i] = i < n ? mask[i < here ? i : a.mask_stride - width + i] : 0;
+      }
+    }
+    const RowGrad r = row_grad(a, row);
+    if (here >= V) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = logit_grad(r, d[i], c + i, scale, inv_t);
+    } else {
+      const RowGrad next = row_grad(a, here < n ? row + 1 : row);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        d[i] = i < here ? logit_grad(r, d[i], c + i, scale, inv_t)
+                        : logit_grad(next, d[i], i - here, scale, inv_t);
+    }
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = allowed[i] ? d[i] : 0.f;
+    }
+    if (n == V) {
       store_run<T, V>(out, d);
     } else {
-      for (int i = 0; i < V && base + o + i < total; ++i) {
-        float x = logit_grad(r, (float)((const T*)a.logits)[row * a.stride + c], c,
-                             inv_t);
-        if (a.mask && !a.mask[row * a.mask_stride + c]) x = 0.f;
-        out[i] = (T)x;
-        if (++c == a.width && row + 1 < a.rows) {
-          c = 0;
-          r = row_grad(a, ++row);
-        }
-      }
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < n) out[i] = (T)d[i];
     }
   }
 }
 
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, bool NARROW = false>
+void fwd_small(const LogProbs& a, hipStream_t stream) {
+  const int64_t need = (a.rows + 256 / TPR - 1) / (256 / TPR);
+  const dim3 grid((unsigned)(need < (1 << 20) ? need : (1 << 20)));
+  logprobs_small_kernel<T, TPR, NV, NARROW><<<grid, 256, 0, stream>>>(a);
+}
+
+template <typename T, int TPR>
 void fwd_as(const LogProbs& a, hipStream_t stream) {
-  constexpr int rpb = TPR > 64 ? 1 : 256 / TPR;
+  const int64_t rpb = TPR > 64 ? 1 : 256 / TPR;
   const int64_t need = (a.rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(need < (1 << 20) ? need : (1 << 20)));
-  logprobs_kernel<T, TPR, NV><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
+  logprobs_kernel<T, TPR><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
 }
 
 template <typename T>
 void fwd(const LogProbs& a, hipStream_t stream) {
   const int n = (a.width + Width<T>::v - 1) / Width<T>::v;    // runs of 16 bytes
-  if (n <= 8 && !a.top_k) fwd_as<T, 8, 1>(a, stream);
-  else if (n <= 64) fwd_as<T, 64, 1>(a, stream);
-  else if (n <= 128) fwd_as<T, 64, 2>(a, stream);
-  else if (n <= 256) fwd_as<T, 64, 4>(a, stream);
-  else if (n <= 512) fwd_as<T, 256, 2>(a, stream);
-  else if (n <= 1024) fwd_as<T, 256, 4>(a, stream);
-  else if (n <= 2048) fwd_as<T, 1024, 2>(a, stream);
-  else if (n <= 4096) fwd_as<T, 1024, 4>(a, stream);
-  else if (sizeof(T) == 4 && n <= 8192) fwd_as<T, 1024, sizeof(T) == 4 ? 8 : 4>(a, stream);
-  else fwd_as<T, 1024, 0>(a, stream);
+  if (!a.top_k && n <= 128) {
+    if (a.width < Width<T>::v) fwd_small<T, 8, 1, true>(a, stream);
+    else if (n <= 8) fwd_small<T, 8, 1>(a, stream);
+    else if (n <= 16) fwd_small<T, 16, 1>(a, stream);
+    else if (n <= 32) fwd_small<T, 16, 2>(a, stream);
+    else if (n <= 48) fwd_small<T, 16, 3>(a, stream);
+    else if (n <= 80) fwd_small<T, 16, 5>(a, stream);
+    else fwd_small<T, 16, 8>(a, stream);
+  } else if (n <= 256) {
+    fwd_as<T, 64>(a, stream);
+  } else if (n <= 1024 || a.rows >= 512) {
+    fwd_as<T, 256>(a, stream);
+  } else {
+    fwd_as<T, 1024>(a, stream);
+  }
 }
 
 template <typename T>
