@@ -9,7 +9,7 @@
 // Forward, a thread runs through its part of the row with a maximum of its own
 // that its sums follow, four 16-byte runs at a time with the next four under way;
 // the threads' maxima and sums are joined at the end, so a row is read once and
-// waits once. 64, 256 or 1024 threads take a row. Narrow rows without alternatives
+// waits once. 64, 256 or 512 threads take a row. Narrow rows without alternatives
 // lie in the registers of 8 or 16 threads instead.
 //
 // The k alternatives: of 64 maxima over disjoint parts of the row (one of each
@@ -78,6 +78,36 @@ __device__ __forceinline__ Run<T> load_masked(const T* l, const uint8_t* mask,
   return v;
 }
 
+// -inf in the places of v whose byte of q is 0
+template <typename T>
+__device__ __forceinline__ Run<T> masked(Run<T> v, uint64_t q) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+  const uint32_t half[2] = {(uint32_t)q, (uint32_t)(q >> 32)};
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    if constexpr (sizeof(T) == 4) {
+      u[d] = half[0] & (0xffu << 8 * d) ? u[d] : 0xff800000u;
+    } else {
+      const uint32_t two = half[d >> 1] >> 16 * (d & 1);
+      const uint32_t keep = (two & 0xffu ? 0xffffu : 0u) | (two & 0xff00u ? 0xffff0000u : 0u);
+      const uint32_t inf = (uint32_t)__builtin_bit_cast(uint16_t, (T)-kInf) * 0x10001u;
+      u[d] = (u[d] & keep) | (inf & ~keep);
+    }
+  }
+  return __builtin_bit_cast(Run<T>, u);
+}
+
+// Nothing computed from v before this is kept for after it: the compiler would
+// hold every element's 32-bit form between the maximum and the sums.
+template <typename T>
+__device__ __forceinline__ void forget(Run<T>& v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+  asm volatile("" : "+v"(u));
+  v = __builtin_bit_cast(Run<T>, u);
+}
+
 constexpr int kList = 1024;         // alternatives' candidates of a block
 
 // What the waves of a row exchange.
@@ -93,8 +123,7 @@ struct Shared {
   float best_v[waves];
   int best_i[waves];
   int count[TPR > 64 ? 1 : 4];
-  float list_v[kList];
-  int list_i[kList];
+  struct { float v; int i; } list_of[kList];
 };
 
 template <int TPR>
@@ -111,8 +140,7 @@ __device__ __forceinline__ void row_sync() {
 // What a row's first thread leaves: its results but for the alternatives, and
 // what the backward pass needs. `given` is the token's logit, -inf if masked.
 __device__ __forceinline__ void leave(const LogProbs& a, int64_t row, Stat st,
-                                      float given, float scale) {
-  const int64_t token = a.tokens[row];
+                                      int64_t token, float given, float scale) {
   const bool ignored = token == a.ignore_index;
   const bool inside = token >= 0 && token < a.width;
   const bool empty = st.m == -kInf && st.s == 0.f;
@@ -133,8 +161,8 @@ __device__ __forceinline__ void leave(const LogProbs& a, int64_t row, Stat st,
 }
 
 template <typename T>
-__device__ __forceinline__ float given_logit(const LogProbs& a, int64_t row) {
-  const int64_t token = a.tokens[row];
+__device__ __forceinline__ float given_logit(const LogProbs& a, int64_t row,
+                                             int64_t token) {
   if (token < 0 || token >= a.width) return -kInf;
   if (a.mask && !a.mask[row * a.mask_stride + token]) return -kInf;
   return (float)((const T*)a.logits)[row * a.stride + token];
@@ -153,7 +181,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
     const int64_t row = mine < a.rows ? mine : a.rows - 1;
     const T* l = (const T*)a.logits + row * a.stride;
     const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-    const float given = t == 0 ? given_logit<T>(a, row) : 0.f;
+    const int64_t token = a.tokens[row];
     Run<T> v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -166,16 +194,16 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
         __builtin_memcpy(&v[j], l + run.at, 16);
       }
     }
+    // asked for behind the row, whose loads it would hold up
+    const float given = t == 0 ? given_logit<T>(a, row, token) : 0.f;
     if constexpr (!NARROW) {
       if (mask) {
-        uint8_t q[NV][V];
+        uint64_t q[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          __builtin_memcpy(q[j], mask + RowRun<T>((j * TPR + t) * V, a.width).at, V);
+          __builtin_memcpy(&q[j], mask + RowRun<T>((j * TPR + t) * V, a.width).at, V);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[j][i] = q[j][i] ? v[j][i] : (T)-kInf;
+        for (int j = 0; j < NV; ++j) v[j] = masked<T>(v[j], q[j]);
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -195,6 +223,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (NV > 1 && j * TPR * V >= a.width) break;    // the same for all
+      forget<T>(v[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float y = ((float)v[j][i] - m) * scale, e = exp2_(y);
@@ -204,25 +233,25 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
     }
     st.s = lanes_sum<TPR>(st.s);
     st.u = lanes_sum<TPR>(st.u);
-    if (t == 0 && mine < a.rows) leave(a, row, st, given, scale);
+    if (t == 0 && mine < a.rows) leave(a, row, st, token, given, scale);
   }
 }
 
 constexpr int kBatch = 4;           // runs of a thread under way together
 
 // A thread's runs of a row, TPR runs apart, a batch at a time.
-template <typename T, int TPR>
+template <typename T, int TPR, bool MASKED>
 struct Batch {
   static constexpr int V = Width<T>::v;
   Run<T> v[kBatch];
-  uint64_t q[kBatch];
+  uint64_t q[MASKED ? kBatch : 1];
 
   __device__ __forceinline__ void load(const T* l, const uint8_t* mask, int c0,
                                        int width) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       __builtin_memcpy(&v[j], l + RowRun<T>(c0 + j * TPR * V, width).at, 16);
-    if (mask) {
+    if constexpr (MASKED) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         __builtin_memcpy(&q[j], mask + RowRun<T>(c0 + j * TPR * V, width).at, V);
@@ -230,15 +259,10 @@ struct Batch {
   }
 
   // -inf in the places that the mask or the row's end take away
-  __device__ __forceinline__ void limit(bool masked, int c0, int width) {
+  __device__ __forceinline__ void limit(int c0, int width) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (masked) {
-        uint8_t keep[V];
-        __builtin_memcpy(keep, &q[j], V);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = keep[i] ? v[j][i] : (T)-kInf;
-      }
+      if constexpr (MASKED) v[j] = masked<T>(v[j], q[j]);
       const RowRun<T> run(c0 + j * TPR * V, width);
       if (!run.whole()) {
 #pragma unroll
@@ -248,8 +272,8 @@ struct Batch {
   }
 };
 
-template <typename T, int TPR>
-__global__ __launch_bounds__(TPR > 64 ? TPR : 256)
+template <typename T, int TPR, bool MASKED>
+__global__ __launch_bounds__(TPR > 64 ? TPR : 256, TPR > 256 ? 2 : 4)
 void logprobs_kernel(LogProbs a) {
   constexpr int V = Width<T>::v;
   constexpr int RPB = TPR > 64 ? 1 : 256 / TPR;
@@ -269,7 +293,11 @@ void logprobs_kernel(LogProbs a) {
     const int64_t row = some ? mine : a.rows - 1;
     const T* l = (const T*)a.logits + row * a.stride;
     const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-    const float given = t == 0 ? given_logit<T>(a, row) : 0.f;
+    const int64_t token = a.tokens[row];
+    Batch<T, TPR, MASKED> now;
+    if (!narrow) now.load(l, mask, t * V, width);
+    // asked for behind the row's first part, whose loads it would hold up
+    const float given = t == 0 ? given_logit<T>(a, row, token) : 0.f;
 
     Stat st = {-kInf, 0.f, 0.f};
     auto add = [&](const Run<T>& v, float m) {
@@ -299,11 +327,10 @@ void logprobs_kernel(LogProbs a) {
         add(v, raise(most));
       }
     } else {
-      Batch<T, TPR> now, next;
-      now.load(l, mask, t * V, width);
+      Batch<T, TPR, MASKED> next;
       for (int c = 0; c < width; c += kStep) {
         if (c + kStep < width) next.load(l, mask, c + kStep + t * V, width);
-        now.limit(mask, c + t * V, width);
+        now.limit(c + t * V, width);
         float most = -kInf;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
@@ -313,6 +340,7 @@ void logprobs_kernel(LogProbs a) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
           if (c + j * TPR * V >= width) break;          // the same for all
+          forget<T>(now.v[j]);
           add(now.v[j], m);
         }
         now = next;
@@ -340,7 +368,7 @@ void logprobs_kernel(LogProbs a) {
 #pragma unroll
       for (int w = 0; w < W; ++w) st.s += sh.stat[w].s, st.u += sh.stat[w].u;
     }
-    if (t == 0 && some) leave(a, row, st, given, scale);
+    if (t == 0 && some) leave(a, row, st, token, given, scale);
     if (!a.top_k) {
       if constexpr (TPR > 64) __syncthreads();     // sh is used by the next row
       continue;
@@ -352,13 +380,12 @@ void logprobs_kernel(LogProbs a) {
     const int K = a.top_k;
     float* out_lp = a.top_logprobs + row * K;
     int64_t* out_t = a.top_tokens + row * K;
-    // this thread's part of the row once more
-    auto each = [&](auto f) {
-      for (int c = t * V; c < width; c += TPR * V) {
-        const Run<T> v = load_masked<T>(l + c, mask ? mask + c : nullptr, width - c);
+    // the elements of a run, one by one: what follows is rare, so it is small
+    // rather than fast (a lone row's time is also that of fetching its code)
+    auto each_of = [&](int c, auto f) {
+      const Run<T> v = load_masked<T>(l + c, MASKED ? mask + c : nullptr, width - c);
 #pragma unroll
-        for (int i = 0; i < V; ++i) f((float)v[i], c + i);
-      }
+      for (int i = 0; i < V; ++i) f((float)v[i], c + i);
     };
     // the K-th largest of 64 lanes' maxima
     float bound = most;
@@ -378,26 +405,45 @@ void logprobs_kernel(LogProbs a) {
     }
     row_sync<TPR>();
     if constexpr (TPR > 64) bound = sh.bound;
-    const int base = slot * Shared<TPR>::list;
+    auto* list = sh.list_of + slot * Shared<TPR>::list;
     if (!none && most >= bound)
-      each([&](float x, int c) {
-        if (x >= bound && x > -kInf) {
-          const int n = atomicAdd(&sh.count[slot], 1);
-          if (n < Shared<TPR>::list) {
-            sh.list_v[base + n] = x;
-            sh.list_i[base + n] = c;
+      for (int c0 = t * V; c0 < width; c0 += kStep) {
+        int hit = 1;                      // a narrow row is one run
+        if (!narrow) {
+          hit = 0;
+          now.load(l, mask, c0, width);
+          now.limit(c0, width);
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            float r = -kInf;
+#pragma unroll
+            for (int i = 0; i < V; ++i) r = fmaxf(r, (float)now.v[j][i]);
+            hit |= (r >= bound) << j;
           }
         }
-      });
+        for (; hit; hit &= hit - 1) {
+          const int c = c0 + (__ffs(hit) - 1) * TPR * V;
+          if (c >= width) continue;
+          each_of(c, [&](float x, int i) {
+            if (x >= bound && x > -kInf) {
+              const int n = atomicAdd(&sh.count[slot], 1);
+              if (n < Shared<TPR>::list) {
+                list[n].v = x;
+                list[n].i = i;
+              }
+            }
+          });
+        }
+      }
     row_sync<TPR>();
     const int n = none ? 0 : sh.count[slot];
     if (n <= Shared<TPR>::list) {
       for (int q = t; q < n; q += TPR) {
-        const float x = sh.list_v[base + q];
-        const int c = sh.list_i[base + q];
+        const float x = list[q].v;
+        const int c = list[q].i;
         int rank = 0;
-        for (int o = 0; o < n; ++o)
-          rank += before(sh.list_v[base + o], sh.list_i[base + o], x, c);
+#pragma unroll 4
+        for (int o = 0; o < n; ++o) rank += before(list[o].v, list[o].i, x, c);
         if (rank < K) {
           out_lp[rank] = ((x - st.m) * scale - log2sum) * kLn2;
           out_t[rank] = c;
@@ -415,12 +461,13 @@ void logprobs_kernel(LogProbs a) {
       for (int k = 0; k < K; ++k) {
         float bv = -kInf;
         int bi = INT32_MAX;
-        each([&](float x, int c) {
-          if (x > -kInf && before(last_v, last_i, x, c) && before(x, c, bv, bi)) {
-            bv = x;
-            bi = c;
-          }
-        });
+        for (int c = t * V; c < width; c += TPR * V)
+          each_of(c, [&](float x, int i) {
+            if (x > -kInf && before(last_v, last_i, x, i) && before(x, i, bv, bi)) {
+              bv = x;
+              bi = i;
+            }
+          });
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
           const float ov = __shfl_xor(bv, o, 64);
@@ -580,7 +627,10 @@ void fwd_as(const LogProbs& a, hipStream_t stream) {
   const int64_t rpb = TPR > 64 ? 1 : 256 / TPR;
   const int64_t need = (a.rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(need < (1 << 20) ? need : (1 << 20)));
-  logprobs_kernel<T, TPR><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
+  if (a.mask)
+    logprobs_kernel<T, TPR, true><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
+  else
+    logprobs_kernel<T, TPR, false><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
 }
 
 template <typename T>
@@ -599,7 +649,7 @@ void fwd(const LogProbs& a, hipStream_t stream) {
   } else if (n <= 1024 || a.rows >= 512) {
     fwd_as<T, 256>(a, stream);
   } else {
-    fwd_as<T, 1024>(a, stream);
+    fwd_as<T, 512>(a, stream);
   }
 }
 
