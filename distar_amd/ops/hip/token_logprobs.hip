@@ -273,7 +273,7 @@ struct Batch {
 };
 
 template <typename T, int TPR, bool MASKED>
-__global__ __launch_bounds__(TPR > 64 ? TPR : 256, TPR > 256 ? 2 : 4)
+__global__ __launch_bounds__(TPR > 64 ? TPR : 256, TPR > 256 ? 2 : MASKED ? 3 : 4)
 void logprobs_kernel(LogProbs a) {
   constexpr int V = Width<T>::v;
   constexpr int RPB = TPR > 64 ? 1 : 256 / TPR;
@@ -534,9 +534,11 @@ __device__ __forceinline__ float logit_grad(const RowGrad& r, float l, int c,
   return r.m == -kInf ? 0.f : d * inv_t;      // a row without any token
 }
 
-constexpr int kBwdRuns = 4;           // runs a thread takes
+constexpr int kBwdRuns = 2;           // runs a thread takes
 
-template <typename T>
+// FLAT: logits (and mask) without gaps between rows of at least one run, so that
+// a run is one load whatever rows it holds.
+template <typename T, bool FLAT, bool MASKED>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(LogProbsBwd a,
                                                            Divide by_width) {
   constexpr int V = Width<T>::v;
@@ -546,71 +548,93 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(LogProbsBwd a,
   const int64_t base = (int64_t)blockIdx.x * (256 * V * kBwdRuns);
   const int64_t row_b = base / width;
   const uint32_t off_b = (uint32_t)(base - row_b * width);
+  if constexpr (FLAT) {
+    float d[kBwdRuns][V];
+    uint8_t keep[kBwdRuns][V];
+    RowGrad r[kBwdRuns];
+    int64_t row[kBwdRuns], at[kBwdRuns];
+    int c[kBwdRuns];
 #pragma unroll
-  for (int k = 0; k < kBwdRuns; ++k) {
-    const uint32_t o = (k * 256 + threadIdx.x) * V;
-    const int64_t left = total - (base + o);
-    if (left <= 0) break;
-    const int n = left < V ? (int)left : V;
-    const uint32_t q = over(off_b + o, by_width);
-    const int64_t row = row_b + q;
-    const int c = (int)(off_b + o - q * (uint32_t)width);
-    T* out = (T*)a.dlogits + base + o;
-    if (width < V) {                  // many rows in a run
-      int64_t at = row;
-      int col = c;
-      for (int i = 0; i < n; ++i) {
-        const float x = logit_grad(row_grad(a, at),
-                                   (float)((const T*)a.logits)[at * a.stride + col],
-                                   col, scale, inv_t);
-        out[i] = a.mask && !a.mask[at * a.mask_stride + col] ? (T)0.f : (T)x;
-        if (++col == width) col = 0, ++at;
-      }
-      continue;
-    }
-    // the run's first elements belong to this row, others to the next
-    const int here = width - c;
-    const T* l = (const T*)a.logits + row * a.stride + c;
-    const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride + c : nullptr;
-    float d[V];
-    uint8_t allowed[V];
-    if (n == V && (here >= V || a.stride == width)) {
-      load_run<T, V>(l, d);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        d[i] = i < n ? (float)l[i < here ? i : a.stride - width + i] : 0.f;
-    }
-    if (mask) {
-      if (n == V && (here >= V || a.mask_stride == width)) {
-        __builtin_memcpy(allowed, mask, V);
+    for (int k = 0; k < kBwdRuns; ++k) {
+      // the last run moves back to end with the gradient
+      const int64_t o = base + (k * 256 + threadIdx.x) * V;
+      at[k] = o < total - V ? o : total - V;
+      load_run<T, V>((const T*)a.logits + at[k], d[k]);
+      if constexpr (MASKED) __builtin_memcpy(keep[k], a.mask + at[k], V);
+      if (at[k] >= base) {
+        const uint32_t n = off_b + (uint32_t)(at[k] - base);
+        const uint32_t q = over(n, by_width);
+        row[k] = row_b + q;
+        c[k] = (int)(n - q * (uint32_t)width);
       } else {
+        row[k] = at[k] / width;
+        c[k] = (int)(at[k] - row[k] * width);
+      }
+      r[k] = row_grad(a, row[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kBwdRuns; ++k) {
+      const int64_t o = base + (k * 256 + threadIdx.x) * V;
+      const int here = width - c[k];      // elements of the first row
+      if (here >= V) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          allowed[i] = i < n ? mask[i < here ? i : a.mask_stride - width + i] : 0;
+          d[k][i] = logit_grad(r[k], d[k][i], c[k] + i, scale, inv_t);
+      } else {
+        const RowGrad next = row_grad(a, row[k] + 1);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          d[k][i] = i < here ? logit_grad(r[k], d[k][i], c[k] + i, scale, inv_t)
+                             : logit_grad(next, d[k][i], i - here, scale, inv_t);
+      }
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[k][i] = keep[k][i] ? d[k][i] : 0.f;
+      }
+      if (at[k] == o) {
+        store_run<T, V>((T*)a.dlogits + o, d[k]);
+      } else if (o < total) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (at[k] + i >= o) ((T*)a.dlogits)[at[k] + i] = (T)d[k][i];
       }
     }
-    const RowGrad r = row_grad(a, row);
-    if (here >= V) {
+  } else {
+    for (int k = 0; k < kBwdRuns; ++k) {
+      const uint32_t o = (k * 256 + threadIdx.x) * V;
+      const int64_t left = total - (base + o);
+      if (left <= 0) break;
+      const int n = left < V ? (int)left : V;
+      const uint32_t q = over(off_b + o, by_width);
+      int64_t row = row_b + q;
+      int c = (int)(off_b + o - q * (uint32_t)width);
+      const T* l = (const T*)a.logits + row * a.stride;
+      const uint8_t* mask = a.mask + row * a.mask_stride;
+      RowGrad r = row_grad(a, row);
+      float d[V];
+      if (n == V && c + V <= width) {
+        uint8_t keep[V];
+        load_run<T, V>(l + c, d);
+        if constexpr (MASKED) __builtin_memcpy(keep, mask + c, V);
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = logit_grad(r, d[i], c + i, scale, inv_t);
-    } else {
-      const RowGrad next = row_grad(a, here < n ? row + 1 : row);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        d[i] = i < here ? logit_grad(r, d[i], c + i, scale, inv_t)
-                        : logit_grad(next, d[i], i - here, scale, inv_t);
-    }
-    if (mask) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = allowed[i] ? d[i] : 0.f;
-    }
-    if (n == V) {
-      store_run<T, V>(out, d);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < n) out[i] = (T)d[i];
+        for (int i = 0; i < V; ++i) {
+          d[i] = logit_grad(r, d[i], c + i, scale, inv_t);
+          if constexpr (MASKED) d[i] = keep[i] ? d[i] : 0.f;
+        }
+        store_run<T, V>((T*)a.dlogits + base + o, d);
+      } else {
+        for (int i = 0; i < n; ++i) {
+          float x = logit_grad(r, (float)l[c], c, scale, inv_t);
+          if constexpr (MASKED) x = mask[c] ? x : 0.f;
+          ((T*)a.dlogits)[base + o + i] = (T)x;
+          if (++c == width && i + 1 < n) {
+            c = 0;
+            l += a.stride;
+            if constexpr (MASKED) mask += a.mask_stride;
+            r = row_grad(a, ++row);
+          }
+        }
+      }
     }
   }
 }
@@ -656,9 +680,18 @@ void fwd(const LogProbs& a, hipStream_t stream) {
 template <typename T>
 void bwd(const LogProbsBwd& a, hipStream_t stream) {
   constexpr int64_t chunk = 256 * Width<T>::v * kBwdRuns;
-  const int64_t blocks = (a.rows * a.width + chunk - 1) / chunk;
-  logprobs_bwd_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(
-      a, divide_by((uint32_t)a.width));
+  const dim3 grid((unsigned)((a.rows * a.width + chunk - 1) / chunk));
+  const Divide by = divide_by((uint32_t)a.width);
+  const bool flat = a.width >= Width<T>::v && (a.stride == a.width || a.rows == 1) &&
+                    (!a.mask || a.mask_stride == a.width || a.rows == 1);
+  if (flat && a.mask)
+    logprobs_bwd_kernel<T, true, true><<<grid, 256, 0, stream>>>(a, by);
+  else if (flat)
+    logprobs_bwd_kernel<T, true, false><<<grid, 256, 0, stream>>>(a, by);
+  else if (a.mask)
+    logprobs_bwd_kernel<T, false, true><<<grid, 256, 0, stream>>>(a, by);
+  else
+    logprobs_bwd_kernel<T, false, false><<<grid, 256, 0, stream>>>(a, by);
 }
 
 }  // namespace
