@@ -183,6 +183,33 @@ struct Staged {
   }
 };
 
+// A wave's part of the output from (i0, j0) on: a lane holds 4 consecutive j of
+// one i of each 16 x 16.
+template <typename T, int FI, int FJ>
+__device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ],
+                                    int64_t i0, int64_t j0) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int x = 0; x < FI; ++x) {
+    const int64_t i = i0 + x * 16 + (lane & 15);
+    if (i >= a.i) continue;
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) {
+      const int64_t j = j0 + y * 16 + (lane >> 4) * 4;
+      const int64_t left = a.j - j;
+      if (left <= 0) continue;
+      const int n = left < 4 ? (int)left : 4;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[x][y][e];
+      if (a.partial)
+        store_some<float, 4>(a.partial + (blockIdx.z * a.i + i) * a.j + j, n, v);
+      else
+        finish<T, 4>(a, i, j, n, v);
+    }
+  }
+}
+
 // BI x BJ of the output by WI x WJ waves.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
 __global__ __launch_bounds__(WI * WJ * 64)
@@ -234,26 +261,113 @@ void product_kernel(Product a) {
           acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
     }
   }
-  // a lane holds 4 consecutive j of one i
+  put<T, FI, FJ>(a, acc, i0 + wi, j0 + wj);
+}
+
+// ---- whole chunks: straight from memory into LDS
+
+__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// A tile's loads where every chunk of 8 is wholly inside or outside the operand
+// and aligned. A load writes 16 bytes for each of a wave's lanes, one after the
+// other, so the lane whose bytes land at a place asks for the chunk that belongs
+// there. Chunks behind r's end come from a block of zeros.
+template <typename T, int B, bool TR, int NT>
+struct Direct {
+  using L = Tile<B, TR>;
+  static constexpr int n = L::rows * L::chunks / NT;
+  const T* at[n];
+
+  __device__ __forceinline__ void start(const T* base, int64_t stride, int64_t i0,
+                                        int64_t i_end, int64_t r0) {
 #pragma unroll
-  for (int x = 0; x < FI; ++x) {
-    const int64_t i = i0 + wi + x * 16 + (lane & 15);
-    if (i >= a.i) continue;
-#pragma unroll
-    for (int y = 0; y < FJ; ++y) {
-      const int64_t j = j0 + wj + y * 16 + (lane >> 4) * 4;
-      const int64_t left = a.j - j;
-      if (left <= 0) continue;
-      const int n = left < 4 ? (int)left : 4;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[x][y][e];
-      if (a.partial)
-        store_some<float, 4>(a.partial + (blockIdx.z * a.i + i) * a.j + j, n, v);
-      else
-        finish<T, 4>(a, i, j, n, v);
+    for (int k = 0; k < n; ++k) {
+      const int slot = k * NT + threadIdx.x;
+      const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
+      if constexpr (TR) {
+        int64_t i = i0 + chunk * 8;
+        i = i < i_end ? i : i_end - 8;
+        at[k] = base + (r0 + row) * stride + i;
+      } else {
+        int64_t i = i0 + row;
+        i = i < i_end ? i : i_end - 1;
+        at[k] = base + i * stride + r0 + chunk * 8;
+      }
     }
   }
+
+  // left: how many r there are from the tile's first on
+  __device__ __forceinline__ void load(char* lds, int64_t stride, int64_t left) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const T* p = at[k];
+      if (left < kR) {
+        const int slot = k * NT + threadIdx.x;
+        const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
+        if ((TR ? row : chunk * 8) >= left) p = (const T*)kZeros;
+      }
+      __builtin_amdgcn_global_load_lds((global_ptr)p,
+                                       (lds_ptr)(lds + (k * NT + wave * 64) * 16),
+                                       16, 0, 0);
+      at[k] += TR ? kR * stride : kR;
+    }
+  }
+};
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
+__global__ __launch_bounds__(WI * WJ * 64, 2)
+void product_direct_kernel(Product a) {
+  constexpr int NT = WI * WJ * 64;
+  constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
+  using P = Tile<BI, PT>;
+  using Q = Tile<BJ, QT>;
+  __shared__ __attribute__((aligned(16))) char lds[2][P::bytes + Q::bytes];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i0 = (int64_t)blockIdx.x * BI, j0 = (int64_t)blockIdx.y * BJ;
+  const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
+  const int64_t tiles = (a.r + kR - 1) / kR;
+  const int64_t first = tiles * blockIdx.z / gridDim.z;
+  const int64_t last = tiles * (blockIdx.z + 1) / gridDim.z;
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int x = 0; x < FI; ++x)
+#pragma unroll
+    for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
+  Direct<T, BI, PT, NT> p;
+  Direct<T, BJ, QT, NT> q;
+  p.start((const T*)a.p, a.p_stride, i0, a.i, first * kR);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, first * kR);
+  p.load(lds[0], a.p_stride, a.r - first * kR);
+  q.load(lds[0] + P::bytes, a.q_stride, a.r - first * kR);
+  int now = 0;
+  for (int64_t t = first; t < last; ++t) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (t + 1 < last) {
+      p.load(lds[now ^ 1], a.p_stride, a.r - (t + 1) * kR);
+      q.load(lds[now ^ 1] + P::bytes, a.q_stride, a.r - (t + 1) * kR);
+    }
+#pragma unroll
+    for (int k = 0; k < kR; k += 32) {
+      s16x8 fp[FI], fq[FJ];
+#pragma unroll
+      for (int x = 0; x < FI; ++x) fp[x] = P::fragment(lds[now], wi + x * 16, k);
+#pragma unroll
+      for (int y = 0; y < FJ; ++y)
+        fq[y] = Q::fragment(lds[now] + P::bytes, wj + y * 16, k);
+#pragma unroll
+      for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y)
+          acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
+    }
+    now ^= 1;
+  }
+  put<T, FI, FJ>(a, acc, i0 + wi, j0 + wj);
 }
 
 // the parts of r added up in their order, and the epilogue
@@ -333,11 +447,34 @@ __global__ __launch_bounds__(1024) void bias_join_kernel(ActBwd a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+bool chunked(const void* p, int64_t stride, bool t, int64_t i, int64_t r) {
+  return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && (t ? i : r) % 8 == 0;
+}
+
+bool direct(const Product& a) {
+  return chunked(a.p, a.p_stride, a.p_t, a.i, a.r) &&
+         chunked(a.q, a.q_stride, a.q_t, a.j, a.r);
+}
+
+bool large(const Product& a) {
+  return direct(a) && ceil_div(a.i, 256) * ceil_div(a.j, 256) >= 100;
+}
+
 template <typename T, bool PT, bool QT>
 void launch(const Product& a, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
-                  a.splits);
-  product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
+  if (large(a)) {
+    const dim3 grid((unsigned)ceil_div(a.i, 256), (unsigned)ceil_div(a.j, 256),
+                    a.splits);
+    product_direct_kernel<T, 256, 256, 2, 4, PT, QT><<<grid, 512, 0, stream>>>(a);
+  } else if (direct(a)) {
+    const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
+                    a.splits);
+    product_direct_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
+  } else {
+    const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
+                    a.splits);
+    product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
+  }
   if (a.partial)
     product_join_kernel<T><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 4), 256)),
                              256, 0, stream>>>(a);
@@ -361,6 +498,10 @@ void launch_act_bwd(const ActBwd& a, hipStream_t stream) {
 }  // namespace
 
 int product_splits(const Product& a) {
+  if (large(a)) {
+    const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
+    return tiles <= 128 ? 2 : 1;
+  }
   const int64_t tiles = ceil_div(a.i, 128) * ceil_div(a.j, 128);
   const int64_t deep = ceil_div(a.r, kR);
   int64_t s = 512 / tiles;

@@ -561,6 +561,17 @@ def test_linear_act(device, dtype, rows, k, n):
         _linear_check(x, w, b, act, r if act in (None, 'gelu') or rows % 2 else None, dy)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', LOW)
+@pytest.mark.parametrize('rows,k,n', [(2600, 72, 2568), (520, 2568, 2568), (2600, 2568, 40), (5000, 256, 1024)])
+def test_linear_act_large(dtype, rows, k, n):
+    gen = torch.Generator('cuda').manual_seed(rows + k + n)
+    make = lambda *s: torch.randn(*s, generator=gen, device='cuda').to(dtype)  # noqa: E731
+    x, w, b, dy, r = make(rows, k), (make(n, k) * k ** -0.5).to(dtype), make(n), make(rows, n), make(rows, n)
+    _linear_check(x, w, b, 'gelu', r, dy)
+    _linear_check(x, w, b, 'relu', None, dy)
+
+
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('dtype', LOW)
 def test_linear_act_strides_and_master_weights(device, dtype):
