@@ -183,49 +183,93 @@ struct Staged {
   }
 };
 
-// A wave's part of the output from (i0, j0) on: a lane holds 4 consecutive j of
-// one i of each 16 x 16.
-template <typename T, int FI, int FJ>
+// Which part of the output a block takes. Blocks go to the 8 dies in turn; each
+// die gets a contiguous range of tiles, and neighbours in it form bands of 8
+// tiles of i, so that blocks which run together on a die share operands in its
+// cache.
+struct Place {
+  int i, j, split;
+};
+struct Tiles {
+  int i, j, splits;
+
+  __device__ __forceinline__ Place place(int block) const {
+    const int total = i * j * splits;
+    const int die = block & 7, each = total >> 3, more = total & 7;
+    int n = block >> 3;
+    n += die < more ? die * (each + 1) : more * (each + 1) + (die - more) * each;
+    Place p;
+    p.split = n / (i * j);
+    n -= p.split * (i * j);
+    const int band = n / (8 * j), rest = n - band * 8 * j;
+    const int high = i - band * 8 < 8 ? i - band * 8 : 8;
+    p.j = rest / high;
+    p.i = band * 8 + rest - p.j * high;
+    return p;
+  }
+};
+
+// LDS that a wave needs to put its part of the output, XP x 16 rows at a time.
+template <int FJ, int XP>
+constexpr int put_bytes() { return XP * 16 * (FJ * 16 + 4) * 4; }
+
+// A wave's part of the output from (i0, j0) on. A lane holds 4 consecutive j of
+// one i of each 16 x 16; by way of LDS it gets runs of 8, so that a row's
+// accesses are whole lines and the epilogue is there once.
+template <typename T, int FI, int FJ, int XP>
 __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ],
-                                    int64_t i0, int64_t j0) {
+                                    char* lds, int split, int64_t i0, int64_t j0) {
+  constexpr int kPitch = FJ * 16 + 4;        // floats; 16 rows meet no bank twice
+  constexpr int kLanes = FJ * 2;             // a row's
   const int lane = threadIdx.x & 63;
+  float* const part = (float*)lds;
+  const int64_t j = j0 + lane % kLanes * 8;
+  const int64_t left = a.j - j;
+  const int n = left < 8 ? (int)left : 8;
 #pragma unroll
-  for (int x = 0; x < FI; ++x) {
-    const int64_t i = i0 + x * 16 + (lane & 15);
-    if (i >= a.i) continue;
+  for (int x = 0; x < FI; x += XP) {
 #pragma unroll
-    for (int y = 0; y < FJ; ++y) {
-      const int64_t j = j0 + y * 16 + (lane >> 4) * 4;
-      const int64_t left = a.j - j;
-      if (left <= 0) continue;
-      const int n = left < 4 ? (int)left : 4;
-      float v[4];
+    for (int u = 0; u < XP; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[x][y][e];
+      for (int y = 0; y < FJ; ++y)
+        *(f32x4*)(part + (u * 16 + (lane & 15)) * kPitch + y * 16 + (lane >> 4) * 4) =
+            acc[x + u][y];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int row = lane / kLanes; row < XP * 16; row += 64 / kLanes) {
+      const int64_t i = i0 + x * 16 + row;
+      if (i >= a.i || n <= 0) continue;
+      float v[8];
+      __builtin_memcpy(v, __builtin_assume_aligned(part + row * kPitch +
+                                                   lane % kLanes * 8, 16), 32);
       if (a.partial)
-        store_some<float, 4>(a.partial + (blockIdx.z * a.i + i) * a.j + j, n, v);
+        store_some<float, 8>(a.partial + (split * a.i + i) * a.j + j, n, v);
       else
-        finish<T, 4>(a, i, j, n, v);
+        finish<T, 8>(a, i, j, n, v);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // BI x BJ of the output by WI x WJ waves.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
 __global__ __launch_bounds__(WI * WJ * 64)
-void product_kernel(Product a) {
+void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   using P = Tile<BI, PT>;
   using Q = Tile<BJ, QT>;
   __shared__ __attribute__((aligned(16))) char lds[P::bytes + Q::bytes];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t i0 = (int64_t)blockIdx.x * BI, j0 = (int64_t)blockIdx.y * BJ;
+  const int wave = threadIdx.x >> 6;
+  const Place at = map.place(blockIdx.x);
+  const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
   // this block's part of r, whole tiles
   const int64_t tiles = (a.r + kR - 1) / kR;
-  const int64_t first = tiles * blockIdx.z / gridDim.z;
-  const int64_t last = tiles * (blockIdx.z + 1) / gridDim.z;
+  const int64_t first = tiles * at.split / a.splits;
+  const int64_t last = tiles * (at.split + 1) / a.splits;
   f32x4 acc[FI][FJ];
 #pragma unroll
   for (int x = 0; x < FI; ++x)
@@ -261,7 +305,8 @@ void product_kernel(Product a) {
           acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
     }
   }
-  put<T, FI, FJ>(a, acc, i0 + wi, j0 + wj);
+  __syncthreads();
+  put<T, FI, FJ, 1>(a, acc, lds + wave * put_bytes<FJ, 1>(), at.split, i0 + wi, j0 + wj);
 }
 
 // ---- whole chunks: straight from memory into LDS
@@ -318,20 +363,50 @@ struct Direct {
   }
 };
 
+// Half a tile's (32 r) fragments of a wave.
+template <int BI, int BJ, int FI, int FJ, bool PT, bool QT>
+struct Half {
+  s16x8 p[FI], q[FJ];
+  __device__ __forceinline__ void read(const char* lds, int wi, int wj, int k) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x) p[x] = Tile<BI, PT>::fragment(lds, wi + x * 16, k);
+#pragma unroll
+    for (int y = 0; y < FJ; ++y)
+      q[y] = Tile<BJ, QT>::fragment(lds + Tile<BI, PT>::bytes, wj + y * 16, k);
+  }
+};
+
+// Asks the scheduler to spread READS LDS reads over MMAS matrix instructions.
+template <int READS, int MMAS>
+__device__ __forceinline__ void spread() {
+  constexpr int each = MMAS / READS > 0 ? MMAS / READS : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
+    __builtin_amdgcn_sched_group_barrier(0x008, each, 0);   // matrix instructions
+  }
+}
+
+// Two tiles of LDS, one read while the other is loaded, and two sets of
+// fragments, one multiplied while the other is read. The barrier stands between
+// a tile's halves: behind it the second half is in registers, so the tile's LDS
+// is free for the tile after the next, and there is work while the next tile's
+// first half is read.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
-__global__ __launch_bounds__(WI * WJ * 64, 2)
-void product_direct_kernel(Product a) {
+__global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 2)
+void product_direct_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
-  using P = Tile<BI, PT>;
-  using Q = Tile<BJ, QT>;
-  __shared__ __attribute__((aligned(16))) char lds[2][P::bytes + Q::bytes];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t i0 = (int64_t)blockIdx.x * BI, j0 = (int64_t)blockIdx.y * BJ;
+  constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
+  constexpr int kPBytes = Tile<BI, PT>::bytes;
+  __shared__ __attribute__((aligned(16))) char lds[2][kPBytes + Tile<BJ, QT>::bytes];
+  const int wave = threadIdx.x >> 6;
+  const Place at = map.place(blockIdx.x);
+  const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
   const int64_t tiles = (a.r + kR - 1) / kR;
-  const int64_t first = tiles * blockIdx.z / gridDim.z;
-  const int64_t last = tiles * (blockIdx.z + 1) / gridDim.z;
+  const int64_t first = tiles * at.split / a.splits;
+  const int64_t last = tiles * (at.split + 1) / a.splits;
   f32x4 acc[FI][FJ];
 #pragma unroll
   for (int x = 0; x < FI; ++x)
@@ -341,33 +416,42 @@ void product_direct_kernel(Product a) {
   Direct<T, BJ, QT, NT> q;
   p.start((const T*)a.p, a.p_stride, i0, a.i, first * kR);
   q.start((const T*)a.q, a.q_stride, j0, a.j, first * kR);
-  p.load(lds[0], a.p_stride, a.r - first * kR);
-  q.load(lds[0] + P::bytes, a.q_stride, a.r - first * kR);
+  auto load = [&](int64_t t, int to) {
+    p.load(lds[to], a.p_stride, a.r - t * kR);
+    q.load(lds[to] + kPBytes, a.q_stride, a.r - t * kR);
+  };
+  using H = Half<BI, BJ, FI, FJ, PT, QT>;
+  auto multiply = [&](const H& h) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(h.q[y], h.p[x], acc[x][y], T());
+  };
+  load(first, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (first + 1 < last) load(first + 1, 1);
+  H one, two;
+  one.read(lds[0], wi, wj, 0);
   int now = 0;
   for (int64_t t = first; t < last; ++t) {
+    two.read(lds[now], wi, wj, 32);
+    multiply(one);
+    spread<kReads, FI * FJ>();
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 1 < last) {
-      p.load(lds[now ^ 1], a.p_stride, a.r - (t + 1) * kR);
-      q.load(lds[now ^ 1] + P::bytes, a.q_stride, a.r - (t + 1) * kR);
-    }
-#pragma unroll
-    for (int k = 0; k < kR; k += 32) {
-      s16x8 fp[FI], fq[FJ];
-#pragma unroll
-      for (int x = 0; x < FI; ++x) fp[x] = P::fragment(lds[now], wi + x * 16, k);
-#pragma unroll
-      for (int y = 0; y < FJ; ++y)
-        fq[y] = Q::fragment(lds[now] + P::bytes, wj + y * 16, k);
-#pragma unroll
-      for (int x = 0; x < FI; ++x)
-#pragma unroll
-        for (int y = 0; y < FJ; ++y)
-          acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
-    }
+    if (t + 2 < last) load(t + 2, now);
     now ^= 1;
+    // behind the last tile this reads what is there, and nothing uses it
+    one.read(lds[now], wi, wj, 0);
+    multiply(two);
+    spread<kReads, FI * FJ>();
   }
-  put<T, FI, FJ>(a, acc, i0 + wi, j0 + wj);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  static_assert(WI * WJ * put_bytes<FJ, 2>() <= sizeof(lds), "LDS");
+  put<T, FI, FJ, 2>(a, acc, lds[0] + wave * put_bytes<FJ, 2>(), at.split, i0 + wi,
+                    j0 + wj);
 }
 
 // the parts of r added up in their order, and the epilogue
@@ -462,19 +546,15 @@ bool large(const Product& a) {
 
 template <typename T, bool PT, bool QT>
 void launch(const Product& a, hipStream_t stream) {
-  if (large(a)) {
-    const dim3 grid((unsigned)ceil_div(a.i, 256), (unsigned)ceil_div(a.j, 256),
-                    a.splits);
-    product_direct_kernel<T, 256, 256, 2, 4, PT, QT><<<grid, 512, 0, stream>>>(a);
-  } else if (direct(a)) {
-    const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
-                    a.splits);
-    product_direct_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
-  } else {
-    const dim3 grid((unsigned)ceil_div(a.i, 128), (unsigned)ceil_div(a.j, 128),
-                    a.splits);
-    product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a);
-  }
+  const int side = large(a) ? 256 : 128;
+  const Tiles map = {(int)ceil_div(a.i, side), (int)ceil_div(a.j, side), a.splits};
+  const dim3 grid((unsigned)map.i * map.j * map.splits);
+  if (large(a))
+    product_direct_kernel<T, 256, 256, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
+  else if (direct(a))
+    product_direct_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
+  else
+    product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
   if (a.partial)
     product_join_kernel<T><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 4), 256)),
                              256, 0, stream>>>(a);
