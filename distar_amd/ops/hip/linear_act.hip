@@ -17,7 +17,9 @@
 namespace blk {
 namespace {
 
-constexpr int kR = 64;            // r a tile
+constexpr int kR = 64;            // r a tile, by way of registers
+constexpr int kDR = 32;           // r a tile, straight into LDS
+constexpr int kStages = 4;        // such tiles in LDS
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -37,10 +39,29 @@ __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c, f16) {
 
 // ---- epilogue
 
+// The normal distribution's cdf; e becomes exp(-z^2 / 2). The rational form
+// 7.1.26 of Abramowitz and Stegun's handbook, erfc(x) = poly(1 / (1 + p x))
+// exp(-x^2) for x >= 0, is off by at most 1.5e-7, an eighth of fp16's half step
+// below 1, at a third of erff's instructions.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678f;
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+  float s = fmaf(1.061405429f, t, -1.453152027f);
+  s = fmaf(s, t, 1.421413741f);
+  s = fmaf(s, t, -0.284496736f);
+  s = fmaf(s, t, 0.254829592f);
+  const float tail = 0.5f * s * t * e;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == kRelu) return z < 0.f ? 0.f : z;       // keeps a NaN
-  if constexpr (ACT == kGelu) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if constexpr (ACT == kGelu) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
   if constexpr (ACT == kSilu) return z / (1.f + __expf(-z));
   return z;
 }
@@ -48,9 +69,11 @@ __device__ __forceinline__ float act(float z) {
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == kRelu) return z > 0.f ? 1.f : 0.f;
-  if constexpr (ACT == kGelu)
-    return 0.5f * (1.f + erff(z * 0.70710678f)) +
-           z * __expf(-0.5f * z * z) * 0.3989422804f;
+  if constexpr (ACT == kGelu) {
+    float e;
+    const float cdf = normal_cdf(z, e);
+    return fmaf(z * 0.3989422804f, e, cdf);
+  }
   if constexpr (ACT == kSilu) {
     const float g = 1.f / (1.f + __expf(-z));
     return g * (1.f + z * (1.f - g));
@@ -93,21 +116,23 @@ __device__ __forceinline__ void finish(const Product& a, int64_t i, int64_t j,
 
 // ---- tiles
 
-// An operand's tile in LDS: ROWS rows of CHUNKS chunks of 8 elements. With r
-// contiguous a row is one i and holds 64 r; otherwise a row is one r and holds
+// An operand's tile of B i by KR r in LDS: rows of chunks of 8 elements. With r
+// contiguous a row is one i and holds KR r; otherwise a row is one r and holds
 // the tile's B values of i.
-template <int B, bool TR>
+template <int B, bool TR, int KR>
 struct Tile {
-  static constexpr int rows = TR ? kR : B;
-  static constexpr int chunks = TR ? B / 8 : kR / 8;
+  static constexpr int rows = TR ? KR : B;
+  static constexpr int chunks = TR ? B / 8 : KR / 8;
   static constexpr int bytes = rows * chunks * 16;
 
   // the chunk's place in its row
   static __device__ __forceinline__ int place(int row, int chunk) {
     if constexpr (TR)    // pairs of chunks move together: a read takes 32 bytes
       return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
-    else
+    else if constexpr (KR == 64)
       return chunk ^ ((row >> 1) & 7);
+    else
+      return chunk ^ (-(row >> 2) & 3);
   }
 
   // 8 consecutive r from r0 + 8 (lane / 16) of i = i0 + lane % 16
@@ -138,7 +163,7 @@ struct Tile {
 // Loads of a tile into registers, each thread N chunks, and from there to LDS.
 template <typename T, int B, bool TR, int NT>
 struct Staged {
-  using L = Tile<B, TR>;
+  using L = Tile<B, TR, kR>;
   static constexpr int n = L::rows * L::chunks / NT;
   s16x8 v[n];
 
@@ -259,8 +284,8 @@ __global__ __launch_bounds__(WI * WJ * 64)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
-  using P = Tile<BI, PT>;
-  using Q = Tile<BJ, QT>;
+  using P = Tile<BI, PT, kR>;
+  using Q = Tile<BJ, QT, kR>;
   __shared__ __attribute__((aligned(16))) char lds[P::bytes + Q::bytes];
   const int wave = threadIdx.x >> 6;
   const Place at = map.place(blockIdx.x);
@@ -313,8 +338,18 @@ void product_kernel(Product a, Tiles map) {
 
 __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-typedef const __attribute__((address_space(1))) void* global_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr;
+// 16 bytes for each lane from base + offset into LDS, lane after lane from `lds`
+// on (the same for all lanes, as is base). Written out because behind the builtin
+// the compiler waits for every load under way before it reads LDS at all; these
+// loads write no register, and the kernel counts and waits for them itself.
+__device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :: "v"(from), "s"(lds) : "memory");
+}
 
 // A tile's loads where every chunk of 8 is wholly inside or outside the operand
 // and aligned. A load writes 16 bytes for each of a wave's lanes, one after the
@@ -322,57 +357,61 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 // there. Chunks behind r's end come from a block of zeros.
 template <typename T, int B, bool TR, int NT>
 struct Direct {
-  using L = Tile<B, TR>;
+  using L = Tile<B, TR, kDR>;
   static constexpr int n = L::rows * L::chunks / NT;
-  const T* at[n];
+  const T* tile;              // the same for all lanes; moves on with each tile
+  uint32_t offset[n];         // bytes from there; stays
 
   __device__ __forceinline__ void start(const T* base, int64_t stride, int64_t i0,
                                         int64_t i_end, int64_t r0) {
+    tile = TR ? base + r0 * stride + i0 : base + i0 * stride + r0;
 #pragma unroll
     for (int k = 0; k < n; ++k) {
       const int slot = k * NT + threadIdx.x;
       const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
+      int64_t at;
       if constexpr (TR) {
-        int64_t i = i0 + chunk * 8;
-        i = i < i_end ? i : i_end - 8;
-        at[k] = base + (r0 + row) * stride + i;
+        const int64_t last = i_end - 8 - i0;
+        at = row * stride + (chunk * 8 < last ? chunk * 8 : last);
       } else {
-        int64_t i = i0 + row;
-        i = i < i_end ? i : i_end - 1;
-        at[k] = base + i * stride + r0 + chunk * 8;
+        const int64_t last = i_end - 1 - i0;
+        at = (row < last ? row : last) * stride + chunk * 8;
       }
+      offset[k] = (uint32_t)(at * sizeof(T));
     }
   }
 
   // left: how many r there are from the tile's first on
-  __device__ __forceinline__ void load(char* lds, int64_t stride, int64_t left) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ __forceinline__ void load(uint32_t lds, int64_t stride, int64_t left) {
+    lds += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    if (left >= kDR) {
 #pragma unroll
-    for (int k = 0; k < n; ++k) {
-      const T* p = at[k];
-      if (left < kR) {
+      for (int k = 0; k < n; ++k) to_lds(tile, offset[k], lds + k * NT * 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
         const int slot = k * NT + threadIdx.x;
         const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
-        if ((TR ? row : chunk * 8) >= left) p = (const T*)kZeros;
+        const char* p = (TR ? row : chunk * 8) < left ? (const char*)tile + offset[k]
+                                                      : (const char*)kZeros;
+        to_lds(p, lds + k * NT * 16);
       }
-      __builtin_amdgcn_global_load_lds((global_ptr)p,
-                                       (lds_ptr)(lds + (k * NT + wave * 64) * 16),
-                                       16, 0, 0);
-      at[k] += TR ? kR * stride : kR;
     }
+    tile += TR ? kDR * stride : kDR;
   }
 };
 
-// Half a tile's (32 r) fragments of a wave.
+// A tile's fragments of a wave.
 template <int BI, int BJ, int FI, int FJ, bool PT, bool QT>
-struct Half {
+struct Fragments {
   s16x8 p[FI], q[FJ];
-  __device__ __forceinline__ void read(const char* lds, int wi, int wj, int k) {
+  __device__ __forceinline__ void read(const char* lds, int wi, int wj) {
 #pragma unroll
-    for (int x = 0; x < FI; ++x) p[x] = Tile<BI, PT>::fragment(lds, wi + x * 16, k);
+    for (int x = 0; x < FI; ++x)
+      p[x] = Tile<BI, PT, kDR>::fragment(lds, wi + x * 16, 0);
 #pragma unroll
     for (int y = 0; y < FJ; ++y)
-      q[y] = Tile<BJ, QT>::fragment(lds + Tile<BI, PT>::bytes, wj + y * 16, k);
+      q[y] = Tile<BJ, QT, kDR>::fragment(lds + Tile<BI, PT, kDR>::bytes, wj + y * 16, 0);
   }
 };
 
@@ -387,26 +426,32 @@ __device__ __forceinline__ void spread() {
   }
 }
 
-// Two tiles of LDS, one read while the other is loaded, and two sets of
-// fragments, one multiplied while the other is read. The barrier stands between
-// a tile's halves: behind it the second half is in registers, so the tile's LDS
-// is free for the tile after the next, and there is work while the next tile's
-// first half is read.
+// Four tiles of LDS under way and two sets of fragments, one multiplied while the
+// other is read. A step's barrier says that the next tile has arrived, and that
+// this one is in registers, so that its LDS can take the tile four further on.
+// Every step loads a tile, zeros behind the last, so that a fixed number of
+// loads is under way and a wait can leave the youngest two tiles' alone.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
 __global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 2)
 void product_direct_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
-  constexpr int kPBytes = Tile<BI, PT>::bytes;
-  __shared__ __attribute__((aligned(16))) char lds[2][kPBytes + Tile<BJ, QT>::bytes];
+  constexpr int kPBytes = Tile<BI, PT, kDR>::bytes;
+  constexpr int kBytes = kPBytes + Tile<BJ, QT, kDR>::bytes;
+  constexpr int kLoads = Direct<T, BI, PT, NT>::n + Direct<T, BJ, QT, NT>::n;
+  // s_waitcnt: at most two tiles' loads under way, no LDS read
+  constexpr int kLeave = 2 * kLoads;
+  constexpr int kWait = (kLeave & 15) | (kLeave >> 4) << 14 | 7 << 4;
+  static_assert(kStages == 4 && kLeave < 64, "waits");
+  __shared__ __attribute__((aligned(16))) char lds[kStages * kBytes];
   const int wave = threadIdx.x >> 6;
   const Place at = map.place(blockIdx.x);
   const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
-  const int64_t tiles = (a.r + kR - 1) / kR;
-  const int64_t first = tiles * at.split / a.splits;
-  const int64_t last = tiles * (at.split + 1) / a.splits;
+  const int tiles = (int)((a.r + kDR - 1) / kDR);
+  const int first = (int)((int64_t)tiles * at.split / a.splits);
+  const int count = (int)((int64_t)tiles * (at.split + 1) / a.splits) - first;
   f32x4 acc[FI][FJ];
 #pragma unroll
   for (int x = 0; x < FI; ++x)
@@ -414,44 +459,50 @@ void product_direct_kernel(Product a, Tiles map) {
     for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
   Direct<T, BI, PT, NT> p;
   Direct<T, BJ, QT, NT> q;
-  p.start((const T*)a.p, a.p_stride, i0, a.i, first * kR);
-  q.start((const T*)a.q, a.q_stride, j0, a.j, first * kR);
-  auto load = [&](int64_t t, int to) {
-    p.load(lds[to], a.p_stride, a.r - t * kR);
-    q.load(lds[to] + kPBytes, a.q_stride, a.r - t * kR);
+  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kDR);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kDR);
+  int64_t left = a.r - (int64_t)first * kDR;
+  const int64_t over = left - (int64_t)count * kDR;      // another block's
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  int stage = 0;                                         // the next load's
+  auto load = [&]() {
+    const int64_t mine = left - (over > 0 ? over : 0);
+    p.load(lds0 + stage, a.p_stride, mine);
+    q.load(lds0 + stage + kPBytes, a.q_stride, mine);
+    left -= kDR;
+    stage = stage == (kStages - 1) * kBytes ? 0 : stage + kBytes;
   };
-  using H = Half<BI, BJ, FI, FJ, PT, QT>;
-  auto multiply = [&](const H& h) {
+  using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
+  int ready = kBytes;                                    // the tile to read next
+  auto step = [&](const F& now, F& next) {
+    __builtin_amdgcn_s_waitcnt(kWait);
+    __syncthreads();
+    load();
+    next.read(lds + ready, wi, wj);
+    ready = ready == (kStages - 1) * kBytes ? 0 : ready + kBytes;
 #pragma unroll
     for (int x = 0; x < FI; ++x)
 #pragma unroll
-      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(h.q[y], h.p[x], acc[x][y], T());
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(now.q[y], now.p[x], acc[x][y], T());
+    spread<kReads, FI * FJ>();
   };
-  load(first, 0);
-  __builtin_amdgcn_s_waitcnt(0);
+  F one, two;
+#pragma unroll 1
+  for (int k = 0; k < kStages; ++k) load();
+  // the first of the four; the loop's wait counts from three under way
+  __builtin_amdgcn_s_waitcnt((3 * kLoads & 15) | (3 * kLoads >> 4) << 14 | 7 << 4);
   __syncthreads();
-  if (first + 1 < last) load(first + 1, 1);
-  H one, two;
-  one.read(lds[0], wi, wj, 0);
-  int now = 0;
-  for (int64_t t = first; t < last; ++t) {
-    two.read(lds[now], wi, wj, 32);
-    multiply(one);
-    spread<kReads, FI * FJ>();
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (t + 2 < last) load(t + 2, now);
-    now ^= 1;
-    // behind the last tile this reads what is there, and nothing uses it
-    one.read(lds[now], wi, wj, 0);
-    multiply(two);
-    spread<kReads, FI * FJ>();
+  one.read(lds, wi, wj);
+  int t = 0;
+  for (; t + 2 <= count; t += 2) {
+    step(one, two);
+    step(two, one);
   }
+  if (t < count) step(one, two);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   static_assert(WI * WJ * put_bytes<FJ, 2>() <= sizeof(lds), "LDS");
-  put<T, FI, FJ, 2>(a, acc, lds[0] + wave * put_bytes<FJ, 2>(), at.split, i0 + wi,
-                    j0 + wj);
+  put<T, FI, FJ, 2>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi, j0 + wj);
 }
 
 // the parts of r added up in their order, and the epilogue
@@ -532,7 +583,9 @@ __global__ __launch_bounds__(1024) void bias_join_kernel(ActBwd a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool chunked(const void* p, int64_t stride, bool t, int64_t i, int64_t r) {
-  return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && (t ? i : r) % 8 == 0;
+  // a tile's offsets are 32-bit
+  return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && stride < (1 << 22) &&
+         (t ? i : r) % 8 == 0;
 }
 
 bool direct(const Product& a) {
