@@ -11,6 +11,8 @@
 // banks; an operand with r across its rows is turned by the transposing LDS
 // read. What lies beyond r's end is loaded as zero on both sides, what lies
 // beyond i or j is loaded from a valid place and not stored.
+#include <type_traits>
+
 #include "block_common.h"
 #include "block_ops.h"
 
@@ -81,37 +83,58 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.f;
 }
 
-template <int N>
-__device__ __forceinline__ void apply_act(int which, float (&v)[N]) {
+// What an epilogue does: an Act with bias, z and residual, or nothing.
+constexpr int kPlain = -1;
+
+// The values of out[i][j ... j + 8), of which n exist: bias and residual are
+// loaded by the caller, which has many rows of them under way.
+template <typename T, int EPI>
+__device__ __forceinline__ void finish(const Product& a, int64_t i, int64_t j, int n,
+                                       float (&v)[8], const float (&bias)[8],
+                                       s16x8 residual) {
+  const int64_t at = i * a.j + j;
+  if constexpr (EPI != kPlain) {
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    v[e] = which == kRelu ? act<kRelu>(v[e])
-         : which == kGelu ? act<kGelu>(v[e])
-         : which == kSilu ? act<kSilu>(v[e]) : v[e];
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
+    if (a.z) store_some<T, 8>((T*)a.z + at, n, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = act<EPI>(v[e]);
+    if (a.residual) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const short bits = residual[e];
+        v[e] += (float)__builtin_bit_cast(T, bits);
+      }
+    }
+  }
+  if (a.out_f32) store_some<float, 8>((float*)a.out + at, n, v);
+  else store_some<T, 8>((T*)a.out + at, n, v);
 }
 
-// the values of out[i][j ... j + N), of which n exist
-template <typename T, int N>
-__device__ __forceinline__ void finish(const Product& a, int64_t i, int64_t j,
-                                       int n, float (&v)[N]) {
-  const int64_t at = i * a.j + j;
-  if (a.bias) {
-    float b[N];
-    if (a.bias_f32) load_some<float, N>((const float*)a.bias + j, n, b, 0.f);
-    else load_some<T, N>((const T*)a.bias + j, n, b, 0.f);
+template <typename T>
+__device__ __forceinline__ void load_bias(const Product& a, int64_t j, int n,
+                                          float (&b)[8]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += b[e];
-  }
-  if (a.z) store_some<T, N>((T*)a.z + at, n, v);
-  if (a.act) apply_act<N>(a.act, v);
-  if (a.residual) {
-    float r[N];
-    load_some<T, N>((const T*)a.residual + i * a.residual_stride + j, n, r, 0.f);
+  for (int e = 0; e < 8; ++e) b[e] = 0.f;
+  if (!a.bias || n <= 0) return;
+  if (a.bias_f32) load_some<float, 8>((const float*)a.bias + j, n, b, 0.f);
+  else load_some<T, 8>((const T*)a.bias + j, n, b, 0.f);
+}
+
+template <typename T>
+__device__ __forceinline__ s16x8 load_residual(const Product& a, int64_t i, int64_t j,
+                                               int n) {
+  s16x8 r = (s16x8)0;
+  if (i >= a.i || n <= 0) return r;
+  const short* p = (const short*)a.residual + i * a.residual_stride + j;
+  if (n >= 8) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += r[e];
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r[e] = p[e];
   }
-  if (a.out_f32) store_some<float, N>((float*)a.out + at, n, v);
-  else store_some<T, N>((T*)a.out + at, n, v);
+  return r;
 }
 
 // ---- tiles
@@ -241,16 +264,27 @@ constexpr int put_bytes() { return XP * 16 * (FJ * 16 + 4) * 4; }
 // A wave's part of the output from (i0, j0) on. A lane holds 4 consecutive j of
 // one i of each 16 x 16; by way of LDS it gets runs of 8, so that a row's
 // accesses are whole lines and the epilogue is there once.
-template <typename T, int FI, int FJ, int XP>
+template <typename T, int FI, int FJ, int XP, int EPI>
 __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ],
                                     char* lds, int split, int64_t i0, int64_t j0) {
   constexpr int kPitch = FJ * 16 + 4;        // floats; 16 rows meet no bank twice
   constexpr int kLanes = FJ * 2;             // a row's
+  constexpr int kRows = 64 / kLanes;         // that a wave takes at once
+  constexpr int kGroup = XP * 16 / kRows < 4 ? XP * 16 / kRows : 4;
   const int lane = threadIdx.x & 63;
   float* const part = (float*)lds;
   const int64_t j = j0 + lane % kLanes * 8;
   const int64_t left = a.j - j;
   const int n = left < 8 ? (int)left : 8;
+  float bias[8];
+  s16x8 residual[kGroup];                    // the group's that comes next
+  const bool more = EPI != kPlain && a.residual;
+  if constexpr (EPI != kPlain) load_bias<T>(a, j, n, bias);
+#pragma unroll
+  for (int g = 0; g < kGroup; ++g) {
+    residual[g] = (s16x8)0;
+    if (more) residual[g] = load_residual<T>(a, i0 + g * kRows + lane / kLanes, j, n);
+  }
 #pragma unroll
   for (int x = 0; x < FI; x += XP) {
 #pragma unroll
@@ -262,16 +296,29 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-    for (int row = lane / kLanes; row < XP * 16; row += 64 / kLanes) {
-      const int64_t i = i0 + x * 16 + row;
-      if (i >= a.i || n <= 0) continue;
-      float v[8];
-      __builtin_memcpy(v, __builtin_assume_aligned(part + row * kPitch +
-                                                   lane % kLanes * 8, 16), 32);
-      if (a.partial)
-        store_some<float, 8>(a.partial + (split * a.i + i) * a.j + j, n, v);
-      else
-        finish<T, 8>(a, i, j, n, v);
+    for (int row0 = 0; row0 < XP * 16; row0 += kGroup * kRows) {
+      s16x8 r[kGroup];
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) r[g] = residual[g];
+      if (more) {
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g)
+          residual[g] = load_residual<T>(
+              a, i0 + x * 16 + row0 + (kGroup + g) * kRows + lane / kLanes, j, n);
+      }
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) {
+        const int row = row0 + g * kRows + lane / kLanes;
+        const int64_t i = i0 + x * 16 + row;
+        float v[8];
+        __builtin_memcpy(v, __builtin_assume_aligned(part + row * kPitch +
+                                                     lane % kLanes * 8, 16), 32);
+        if (i >= a.i || n <= 0) continue;
+        if (EPI == kPlain && a.partial)
+          store_some<float, 8>(a.partial + (split * a.i + i) * a.j + j, n, v);
+        else
+          finish<T, EPI>(a, i, j, n, v, bias, r[g]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -279,7 +326,7 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
 }
 
 // BI x BJ of the output by WI x WJ waves.
-template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ __launch_bounds__(WI * WJ * 64)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
@@ -331,7 +378,7 @@ void product_kernel(Product a, Tiles map) {
     }
   }
   __syncthreads();
-  put<T, FI, FJ, 1>(a, acc, lds + wave * put_bytes<FJ, 1>(), at.split, i0 + wi, j0 + wj);
+  put<T, FI, FJ, 1, EPI>(a, acc, lds + wave * put_bytes<FJ, 1>(), at.split, i0 + wi, j0 + wj);
 }
 
 // ---- whole chunks: straight from memory into LDS
@@ -431,7 +478,7 @@ __device__ __forceinline__ void spread() {
 // this one is in registers, so that its LDS can take the tile four further on.
 // Every step loads a tile, zeros behind the last, so that a fixed number of
 // loads is under way and a wait can leave the youngest two tiles' alone.
-template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT>
+template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 2)
 void product_direct_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
@@ -502,58 +549,78 @@ void product_direct_kernel(Product a, Tiles map) {
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   static_assert(WI * WJ * put_bytes<FJ, 2>() <= sizeof(lds), "LDS");
-  put<T, FI, FJ, 2>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi, j0 + wj);
+  put<T, FI, FJ, 2, EPI>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi, j0 + wj);
 }
 
 // the parts of r added up in their order, and the epilogue
-template <typename T>
+template <typename T, int EPI>
 __global__ __launch_bounds__(256) void product_join_kernel(Product a) {
-  const int64_t runs = (a.j + 3) / 4;
+  const int64_t runs = (a.j + 7) / 8;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= a.i * runs) return;
-  const int64_t i = at / runs, j = at % runs * 4;
-  const int n = a.j - j < 4 ? (int)(a.j - j) : 4;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    float q[4];
-    load_some<float, 4>(a.partial + (s * a.i + i) * a.j + j, n, q, 0.f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += q[e];
+  const int64_t i = at / runs, j = at % runs * 8;
+  const int n = a.j - j < 8 ? (int)(a.j - j) : 8;
+  float bias[8], v[8] = {};
+  s16x8 residual = (s16x8)0;
+  if constexpr (EPI != kPlain) {
+    load_bias<T>(a, j, n, bias);
+    if (a.residual) residual = load_residual<T>(a, i, j, n);
   }
-  finish<T, 4>(a, i, j, n, v);
+  const float* p = a.partial + i * a.j + j;
+  const int64_t part = a.i * a.j;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    float q[8];
+    load_some<float, 8>(p + s * part, n, q, 0.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += q[e];
+  }
+  finish<T, EPI>(a, i, j, n, v, bias, residual);
 }
 
 // ---- dz and db
 
-// 32 threads take 8 columns each, 8 rows at a time.
-template <typename T>
+constexpr int kActRows = 4;           // rows of a thread under way together
+
+// 32 threads take 8 columns each, 8 rows at a time. NARROW: fewer than 8 columns.
+template <typename T, int ACT, bool NARROW>
 __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwd a) {
   __shared__ float part[8][257];
   const int t = threadIdx.x & 31, group = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.x * 256 + t * 8;
-  const int64_t left = a.n - j;
-  const int n = left < 8 ? (int)left : 8;
+  const RowRun<T, NARROW> run(blockIdx.x * 256 + t * 8, (int)a.n);
   float db[8] = {};
-  if (n > 0)
-    for (int64_t i = (int64_t)blockIdx.y * 8 + group; i < a.rows;
-         i += (int64_t)gridDim.y * 8) {
-      float d[8], z[8];
-      load_some<T, 8>((const T*)a.dy + i * a.dy_stride + j, n, d, 0.f);
-      if (a.act) {
-        load_some<T, 8>((const T*)a.z + i * a.n + j, n, z, 0.f);
+  if (run.any())
+    for (int64_t i0 = (int64_t)blockIdx.y * 8 * kActRows + group; i0 < a.rows;
+         i0 += (int64_t)gridDim.y * 8 * kActRows) {
+      float d[kActRows][8], z[kActRows][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          d[e] = a.act == kRelu ? (z[e] > 0.f ? d[e] : z[e] != z[e] ? z[e] : 0.f)
-               : a.act == kGelu ? d[e] * act_slope<kGelu>(z[e])
-                                : d[e] * act_slope<kSilu>(z[e]);
-        store_some<T, 8>((T*)a.dz + i * a.n + j, n, d);
+      for (int k = 0; k < kActRows; ++k) {
+        const int64_t i = i0 + k * 8 < a.rows ? i0 + k * 8 : a.rows - 1;
+        run.load((const T*)a.dy + i * a.dy_stride, d[k]);
+        if constexpr (ACT != kNone) run.load((const T*)a.z + i * a.n, z[k]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) db[e] += d[e];
+      for (int k = 0; k < kActRows; ++k) {
+        if (i0 + k * 8 >= a.rows) break;
+        if constexpr (ACT != kNone) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if constexpr (ACT == kRelu)
+              d[k][e] = z[k][e] > 0.f ? d[k][e] : z[k][e] != z[k][e] ? z[k][e] : 0.f;
+            else
+              d[k][e] *= act_slope<ACT>(z[k][e]);
+          }
+          run.store((T*)a.dz + (i0 + k * 8) * a.n, d[k]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) db[e] += d[k][e];
+      }
     }
   if (!a.partial) return;
+  // the run that moved back has some columns twice
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[group][t * 8 + e] = db[e];
+  for (int e = 0; e < 8; ++e)
+    if (run.counts(e)) part[group][run.at + e - blockIdx.x * 256] = db[e];
   __syncthreads();
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (col >= a.n) return;
@@ -570,6 +637,7 @@ __global__ __launch_bounds__(1024) void bias_join_kernel(ActBwd a) {
   const int64_t c = (int64_t)blockIdx.x * 16 + lane;
   float v = 0.f;
   if (c < a.n)
+#pragma unroll 4
     for (int k = group; k < a.blocks; k += 64) v += a.partial[k * a.n + c];
   lds[group][lane] = v;
   __syncthreads();
@@ -597,33 +665,55 @@ bool large(const Product& a) {
   return direct(a) && ceil_div(a.i, 256) * ceil_div(a.j, 256) >= 100;
 }
 
-template <typename T, bool PT, bool QT>
+template <typename T, bool PT, bool QT, int EPI>
 void launch(const Product& a, hipStream_t stream) {
   const int side = large(a) ? 256 : 128;
   const Tiles map = {(int)ceil_div(a.i, side), (int)ceil_div(a.j, side), a.splits};
   const dim3 grid((unsigned)map.i * map.j * map.splits);
   if (large(a))
-    product_direct_kernel<T, 256, 256, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
+    product_direct_kernel<T, 256, 256, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
   else if (direct(a))
-    product_direct_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
+    product_direct_kernel<T, 128, 128, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
   else
-    product_kernel<T, 128, 128, 2, 2, PT, QT><<<grid, 256, 0, stream>>>(a, map);
-  if (a.partial)
-    product_join_kernel<T><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 4), 256)),
-                             256, 0, stream>>>(a);
+    product_kernel<T, 128, 128, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
+}
+
+template <typename T, int EPI>
+void join(const Product& a, hipStream_t stream) {
+  product_join_kernel<T, EPI><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 8), 256)),
+                                256, 0, stream>>>(a);
 }
 
 template <typename T>
 void launch_any(const Product& a, hipStream_t stream) {
-  if (a.p_t) launch<T, true, true>(a, stream);
-  else if (a.q_t) launch<T, false, true>(a, stream);
-  else launch<T, false, false>(a, stream);
+  const bool plain = !a.bias && !a.z && !a.act && !a.residual;
+  if (a.p_t) launch<T, true, true, kPlain>(a, stream);
+  else if (a.q_t) launch<T, false, true, kPlain>(a, stream);
+  else if (plain || a.partial) launch<T, false, false, kPlain>(a, stream);
+  else if (a.act == kNone) launch<T, false, false, kNone>(a, stream);
+  else if (a.act == kRelu) launch<T, false, false, kRelu>(a, stream);
+  else if (a.act == kGelu) launch<T, false, false, kGelu>(a, stream);
+  else launch<T, false, false, kSilu>(a, stream);
+  if (!a.partial) return;
+  if (plain) join<T, kPlain>(a, stream);
+  else if (a.act == kNone) join<T, kNone>(a, stream);
+  else if (a.act == kRelu) join<T, kRelu>(a, stream);
+  else if (a.act == kGelu) join<T, kGelu>(a, stream);
+  else join<T, kSilu>(a, stream);
 }
 
 template <typename T>
 void launch_act_bwd(const ActBwd& a, hipStream_t stream) {
-  act_bwd_kernel<T><<<dim3((unsigned)ceil_div(a.n, 256), a.blocks), 256, 0,
-                      stream>>>(a);
+  const dim3 grid((unsigned)ceil_div(a.n, 256), a.blocks);
+  auto run = [&](auto narrow) {
+    constexpr bool N = decltype(narrow)::value;
+    if (a.act == kNone) act_bwd_kernel<T, kNone, N><<<grid, 256, 0, stream>>>(a);
+    else if (a.act == kRelu) act_bwd_kernel<T, kRelu, N><<<grid, 256, 0, stream>>>(a);
+    else if (a.act == kGelu) act_bwd_kernel<T, kGelu, N><<<grid, 256, 0, stream>>>(a);
+    else act_bwd_kernel<T, kSilu, N><<<grid, 256, 0, stream>>>(a);
+  };
+  if (a.n < 8) run(std::true_type());
+  else run(std::false_type());
   if (a.partial)
     bias_join_kernel<T><<<dim3((unsigned)ceil_div(a.n, 16)), 1024, 0, stream>>>(a);
 }
@@ -649,9 +739,9 @@ void product(const Product& a, int dtype, hipStream_t stream) {
 
 int act_bwd_blocks(int64_t rows, int64_t n) {
   const int64_t wide = ceil_div(n, 256);
-  int64_t b = 2048 / wide;
+  int64_t b = 1024 / wide;
   b = b < 64 ? 64 : b;
-  const int64_t need = ceil_div(rows, 8);
+  const int64_t need = ceil_div(rows, 8 * kActRows);
   return (int)(need < b ? need : b);
 }
 
