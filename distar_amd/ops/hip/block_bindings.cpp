@@ -435,9 +435,21 @@ int linear_dtype(const Tensor& t, const char* name) {
   return d;
 }
 
+// Rows as the products take them: of 8 elements at least, and with a stride that
+// leaves a tile's offsets in 32 bits.
+Rows product_rows_of(const Tensor& in) {
+  if (in.size(-1) < 8) {
+    const Tensor wide = torch::constant_pad_nd(in, {0, 8 - in.size(-1)}, 0);
+    return {wide, wide.numel() / 8, 8};
+  }
+  Rows r = rows_of(in);
+  if (r.stride < 0 || r.stride >= (1 << 22)) r = {in.contiguous(), r.rows, in.size(-1)};
+  return r;
+}
+
 void run_product(blk::Product& a, int dtype, const Tensor& like) {
-  TORCH_CHECK_VALUE(a.i <= (int64_t)1 << 30 && a.j <= (int64_t)1 << 22,
-                    "a product of ", a.i, " by ", a.j, " is too large");
+  TORCH_CHECK_VALUE(a.i < (int64_t)1 << 32 && a.r < (int64_t)1 << 32,
+                    "more than 2^32 rows");
   a.splits = blk::product_splits(a);
   Tensor partial;
   if (a.splits > 1) {
@@ -461,6 +473,8 @@ std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1,
                     "weight must be (outputs, ", x.size(-1), ")");
   const int64_t n = weight.size(0);
+  TORCH_CHECK_VALUE(n < (1 << 22) && x.size(-1) < (1 << 22),
+                    "a layer's widths must be below 2^22");
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = n;
   if (bias.has_value()) {
@@ -477,7 +491,7 @@ std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
                       "residual must be of the output's shape");
   }
   const c10::DeviceGuard guard(x.device());
-  const Rows xr = rows_of(x), wr = rows_of(weight.to(x.scalar_type()));
+  const Rows xr = product_rows_of(x), wr = product_rows_of(weight.to(x.scalar_type()));
   if (bias.has_value()) bias = bias->contiguous();
   const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
   Tensor y = torch::empty(shape, x.options());
@@ -489,6 +503,8 @@ std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
     a.q = wr.t.data_ptr();
     a.p_stride = xr.stride;
     a.q_stride = wr.stride;
+    a.p_cols = xr.t.size(-1);
+    a.q_cols = wr.t.size(-1);
     a.i = xr.rows;
     a.j = n;
     a.r = x.size(-1);
@@ -511,8 +527,8 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
   const int dtype = linear_dtype(x, "x");
   const int64_t n = weight.size(0), k = weight.size(1);
   const c10::DeviceGuard guard(x.device());
-  const Rows yr = rows_of(dy), xr = rows_of(x);
-  const int64_t rows = xr.rows;
+  const Rows yr = rows_of(dy);
+  const int64_t rows = yr.rows;
   Tensor dx, dw, db;
   if (need_x) dx = torch::empty(x.sizes(), x.options());
   if (need_w) dw = torch::empty({n, k}, weight.options());
@@ -524,7 +540,6 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
   }
   const hipStream_t stream = stream_of(x);
   Tensor dz = yr.t;
-  int64_t dz_stride = yr.stride;
   if (act || need_b) {
     blk::ActBwd b{};
     b.blocks = blk::act_bwd_blocks(rows, n);
@@ -534,7 +549,6 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
     b.dy = yr.t.data_ptr();
     if (act) {
       dz = torch::empty({rows, n}, x.options());
-      dz_stride = n;
       b.z = saved.data_ptr();
       b.dz = dz.data_ptr();
     }
@@ -548,13 +562,16 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
     blk::act_bwd(b, dtype, stream);
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
+  const Rows zr = need_x || need_w ? product_rows_of(dz) : Rows{dz, 0, 0};
   if (need_x) {
-    const Rows wr = rows_of(weight.to(x.scalar_type()));
+    const Rows wr = product_rows_of(weight.to(x.scalar_type()));
     blk::Product a{};
-    a.p = dz.data_ptr();
+    a.p = zr.t.data_ptr();
     a.q = wr.t.data_ptr();
-    a.p_stride = dz_stride;
+    a.p_stride = zr.stride;
     a.q_stride = wr.stride;
+    a.p_cols = zr.t.size(-1);
+    a.q_cols = wr.t.size(-1);
     a.i = rows;
     a.j = k;
     a.r = n;
@@ -563,11 +580,14 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
     run_product(a, dtype, x);
   }
   if (need_w) {
+    const Rows xr = product_rows_of(x);
     blk::Product a{};
-    a.p = dz.data_ptr();
+    a.p = zr.t.data_ptr();
     a.q = xr.t.data_ptr();
-    a.p_stride = dz_stride;
+    a.p_stride = zr.stride;
     a.q_stride = xr.stride;
+    a.p_cols = zr.t.size(-1);
+    a.q_cols = xr.t.size(-1);
     a.i = n;
     a.j = k;
     a.r = rows;

@@ -78,6 +78,8 @@ enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
 struct Product {
   const void *p, *q;
   int64_t p_stride, q_stride;
+  int64_t p_cols, q_cols;                     // a row's elements, 8 at least: what
+                                              // lies behind i, j or r is zero
   int64_t i, j, r;
   bool p_t, q_t;
   void *out;                                  // [i][j], contiguous

@@ -5,7 +5,7 @@
 //
 // One kernel does the three products out[i][j] = sum_r P[i][r] Q[j][r] on the
 // matrix cores (16x16x32, 32-bit sums): an operand's r is contiguous in
-// memory, or its other index is (W for dx, both operands for dW). Tiles of 64 r
+// memory, or its other index is (W for dx, both operands for dW). Tiles of 32 r
 // go through LDS as they lie in memory, in 16-byte chunks whose place in their
 // row is XORed with bits of the row, so that the reads of a wave spread over all
 // banks; an operand with r across its rows is turned by the transposing LDS
@@ -19,9 +19,8 @@
 namespace blk {
 namespace {
 
-constexpr int kR = 64;            // r a tile, by way of registers
-constexpr int kDR = 32;           // r a tile, straight into LDS
-constexpr int kStages = 4;        // such tiles in LDS
+constexpr int kR = 32;            // r a tile
+constexpr int kStages = 4;        // tiles in LDS
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -139,28 +138,25 @@ __device__ __forceinline__ s16x8 load_residual(const Product& a, int64_t i, int6
 
 // ---- tiles
 
-// An operand's tile of B i by KR r in LDS: rows of chunks of 8 elements. With r
-// contiguous a row is one i and holds KR r; otherwise a row is one r and holds
+// An operand's tile of B i by 32 r in LDS: rows of chunks of 8 elements. With r
+// contiguous a row is one i and holds 32 r; otherwise a row is one r and holds
 // the tile's B values of i.
-template <int B, bool TR, int KR>
+template <int B, bool TR>
 struct Tile {
-  static constexpr int rows = TR ? KR : B;
-  static constexpr int chunks = TR ? B / 8 : KR / 8;
+  static constexpr int rows = TR ? kR : B;
+  static constexpr int chunks = TR ? B / 8 : kR / 8;
   static constexpr int bytes = rows * chunks * 16;
 
-  // the chunk's place in its row
+  // The chunk's place in its row. A read with r contiguous takes 16 lanes' rows
+  // together, in fours of which two ask for one chunk and two for its neighbour;
+  // a turning read takes 32 bytes, so there pairs of chunks move together.
   static __device__ __forceinline__ int place(int row, int chunk) {
-    if constexpr (TR)    // pairs of chunks move together: a read takes 32 bytes
-      return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
-    else if constexpr (KR == 64)
-      return chunk ^ ((row >> 1) & 7);
-    else
-      return chunk ^ (-(row >> 2) & 3);
+    if constexpr (TR) return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
+    else return chunk ^ (-(row >> 2) & 3);
   }
 
-  // 8 consecutive r from r0 + 8 (lane / 16) of i = i0 + lane % 16
-  static __device__ __forceinline__ s16x8 fragment(const char* lds, int i0,
-                                                   int r0) {
+  // 8 consecutive r from 8 (lane / 16) on of i = i0 + lane % 16
+  static __device__ __forceinline__ s16x8 fragment(const char* lds, int i0) {
     const int lane = threadIdx.x & 63;
     if constexpr (TR) {
       // lanes 4q ... 4q + 3 of 16 fetch row q's 16 elements; lane c gets
@@ -168,7 +164,7 @@ struct Tile {
       s16x4 part[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = r0 + (lane >> 4) * 8 + h * 4 + ((lane >> 2) & 3);
+        const int row = (lane >> 4) * 8 + h * 4 + ((lane >> 2) & 3);
         const int col = i0 + (lane & 3) * 4;
         const char* p = lds + (row * chunks + place(row, col >> 3)) * 16 +
                         (col & 7) * 2;
@@ -177,57 +173,131 @@ struct Tile {
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       const int row = i0 + (lane & 15);
-      const int chunk = (r0 >> 3) + (lane >> 4);
+      const int chunk = lane >> 4;
       return *(const s16x8*)(lds + (row * chunks + place(row, chunk)) * 16);
     }
   }
 };
 
-// Loads of a tile into registers, each thread N chunks, and from there to LDS.
+// A tile's fragments of a wave.
+template <int BI, int BJ, int FI, int FJ, bool PT, bool QT>
+struct Fragments {
+  s16x8 p[FI], q[FJ];
+  __device__ __forceinline__ void read(const char* lds, int wi, int wj) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x) p[x] = Tile<BI, PT>::fragment(lds, wi + x * 16);
+#pragma unroll
+    for (int y = 0; y < FJ; ++y)
+      q[y] = Tile<BJ, QT>::fragment(lds + Tile<BI, PT>::bytes, wj + y * 16);
+  }
+};
+
+// Asks the scheduler to put one of READS LDS reads in front of each of the first
+// matrix instructions. (With the reads spread evenly over all of them, or left to
+// the compiler, the products of 16384 x 4096 x 2048 run at 966 to 1200 TFLOP/s,
+// so at 1142 to 1213.)
+template <int READS, int WRITES = 0>
+__device__ __forceinline__ void spread() {
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    if (i < WRITES) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);   // a write
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                   // a read
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                   // a product
+  }
+}
+
+// A tile's loads by way of registers, at any alignment: each thread N chunks. A
+// chunk that would pass the end of its row is loaded from further left and moved
+// into place on its way to LDS, zeros behind it; so every load is made, without a
+// condition, and waits can count them.
 template <typename T, int B, bool TR, int NT>
 struct Staged {
-  using L = Tile<B, TR, kR>;
+  using L = Tile<B, TR>;
   static constexpr int n = L::rows * L::chunks / NT;
-  s16x8 v[n];
+  const T* tile;              // the same for all lanes; moves on with each tile
+  int32_t offset[n];          // bytes from there; stays
+  int back[n];                // elements that the load starts before its chunk (TR)
+  int64_t columns;            // of a row from the tile's first on (not TR)
 
-  // base: the operand; i0, r0: the tile's origin; i_end, r_end: where it ends
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t i0,
-                                       int64_t i_end, int64_t r0, int64_t r_end) {
+  static __device__ __forceinline__ int row_of(int k) {
+    return (k * NT + threadIdx.x) / L::chunks;
+  }
+  static __device__ __forceinline__ int chunk_of(int k) {
+    return (k * NT + threadIdx.x) % L::chunks;
+  }
+
+  // cols: a row's elements in memory, 8 at least
+  __device__ __forceinline__ void start(const T* base, int64_t stride, int64_t i0,
+                                        int64_t i_end, int64_t r0, int64_t cols) {
+    tile = TR ? base + r0 * stride + i0 : base + i0 * stride + r0;
+    columns = cols - r0;
 #pragma unroll
     for (int k = 0; k < n; ++k) {
-      const int at = k * NT + threadIdx.x;
-      const int row = at / L::chunks, chunk = at % L::chunks;
-      v[k] = (s16x8)0;
+      const int64_t last = TR ? cols - i0 - 8 : i_end - 1 - i0;
+      const int row = row_of(k), chunk = chunk_of(k);
       if constexpr (TR) {
-        const int64_t r = r0 + row;
-        const int64_t some = i_end - (i0 + chunk * 8);
-        if (r < r_end) fetch(base + r * stride + i0 + chunk * 8, some, v[k]);
+        const int at = chunk * 8 < last ? chunk * 8 : (int)last;
+        back[k] = chunk * 8 - at;
+        offset[k] = (int32_t)((row * stride + at) * (int)sizeof(T));
       } else {
-        int64_t i = i0 + row;
-        i = i < i_end ? i : i_end - 1;
-        const int64_t some = r_end - (r0 + chunk * 8);
-        fetch(base + i * stride + r0 + chunk * 8, some, v[k]);
+        const int line = row < last ? row : (int)last;
+        offset[k] = (int32_t)((line * stride + chunk * 8) * (int)sizeof(T));
       }
     }
   }
 
-  static __device__ __forceinline__ void fetch(const T* p, int64_t some, s16x8& o) {
-    if (some >= 8) {
-      __builtin_memcpy(&o, p, 16);
-    } else {
+  // left: how many r there are from the tile's first on; at least 1
+  __device__ __forceinline__ void load(s16x8 (&v)[n], int64_t stride, int64_t left) {
+    int32_t o[n];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < some) o[e] = ((const short*)p)[e];
+    for (int k = 0; k < n; ++k) o[k] = offset[k];
+    if (TR ? left < kR : columns < kR) {
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        if constexpr (TR) {
+          const int over = row_of(k) - ((int)left - 1);
+          if (over > 0) o[k] -= (int32_t)(over * stride * (int)sizeof(T));
+        } else {
+          const int over = chunk_of(k) * 8 - ((int)columns - 8);
+          if (over > 0) o[k] -= over * (int)sizeof(T);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < n; ++k) __builtin_memcpy(&v[k], (const char*)tile + o[k], 16);
+  }
+  __device__ __forceinline__ void next(int64_t stride) {
+    tile += TR ? kR * stride : kR;
+    columns -= kR;
+  }
+
+  // columns_, left: of the tile that v holds
+  __device__ __forceinline__ void store(const s16x8 (&v)[n], char* lds, int64_t left,
+                                        int64_t columns_, bool edge) const {
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const int row = row_of(k), chunk = chunk_of(k);
+      s16x8 x = v[k];
+      if (TR ? edge || left < kR : columns_ < kR) {
+        int by = TR ? back[k] : chunk * 8 - ((int)columns_ - 8);
+        by = by < 0 ? 0 : by > 8 || (TR && row >= left) ? 8 : by;
+        x = moved(x, by);
+      }
+      *(s16x8*)(lds + (row * L::chunks + L::place(row, chunk)) * 16) = x;
     }
   }
 
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int k = 0; k < n; ++k) {
-      const int at = k * NT + threadIdx.x;
-      const int row = at / L::chunks, chunk = at % L::chunks;
-      *(s16x8*)(lds + (row * L::chunks + L::place(row, chunk)) * 16) = v[k];
-    }
+  // x[e + by], zeros behind
+  static __device__ __forceinline__ s16x8 moved(s16x8 x, int by) {
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    u64x2 u = __builtin_bit_cast(u64x2, x);
+    uint64_t lo = u[0], hi = u[1];
+    if (by & 4) lo = hi, hi = 0;
+    const int bits = (by & 3) * 16;
+    const uint64_t carry = bits ? hi << (64 - bits) : 0;
+    u[0] = by >= 8 ? 0 : lo >> bits | carry;
+    u[1] = by >= 8 ? 0 : hi >> bits;
+    return __builtin_bit_cast(s16x8, u);
   }
 };
 
@@ -325,60 +395,95 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
   }
 }
 
-// BI x BJ of the output by WI x WJ waves.
+// BI x BJ of the output by WI x WJ waves, operands at any alignment. While a tile
+// is multiplied, the next one's fragments are read, the one after goes from
+// registers to LDS, and the four after that are under way into four sets of
+// registers.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
-__global__ __launch_bounds__(WI * WJ * 64)
+__global__ __launch_bounds__(WI * WJ * 64, 2)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
-  using P = Tile<BI, PT, kR>;
-  using Q = Tile<BJ, QT, kR>;
-  __shared__ __attribute__((aligned(16))) char lds[P::bytes + Q::bytes];
+  constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
+  constexpr int kPBytes = Tile<BI, PT>::bytes;
+  constexpr int kBytes = kPBytes + Tile<BJ, QT>::bytes;
+  using P = Staged<T, BI, PT, NT>;
+  using Q = Staged<T, BJ, QT, NT>;
+  __shared__ __attribute__((aligned(16))) char lds[kStages * kBytes];
   const int wave = threadIdx.x >> 6;
   const Place at = map.place(blockIdx.x);
   const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
   // this block's part of r, whole tiles
-  const int64_t tiles = (a.r + kR - 1) / kR;
-  const int64_t first = tiles * at.split / a.splits;
-  const int64_t last = tiles * (at.split + 1) / a.splits;
+  const int tiles = (int)((a.r + kR - 1) / kR);
+  const int first = (int)((int64_t)tiles * at.split / a.splits);
+  const int count = (int)((int64_t)tiles * (at.split + 1) / a.splits) - first;
   f32x4 acc[FI][FJ];
 #pragma unroll
   for (int x = 0; x < FI; ++x)
 #pragma unroll
     for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
-  Staged<T, BI, PT, NT> p;
-  Staged<T, BJ, QT, NT> q;
-  if (first < last) {
-    p.load((const T*)a.p, a.p_stride, i0, a.i, first * kR, a.r);
-    q.load((const T*)a.q, a.q_stride, j0, a.j, first * kR, a.r);
-  }
-  for (int64_t t = first; t < last; ++t) {
-    __syncthreads();
-    p.store(lds);
-    q.store(lds + P::bytes);
-    __syncthreads();
-    if (t + 1 < last) {
-      p.load((const T*)a.p, a.p_stride, i0, a.i, (t + 1) * kR, a.r);
-      q.load((const T*)a.q, a.q_stride, j0, a.j, (t + 1) * kR, a.r);
+  P p;
+  Q q;
+  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kR, a.p_cols);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kR, a.q_cols);
+  const bool edge_p = a.p_cols - i0 < BI, edge_q = a.q_cols - j0 < BJ;
+  s16x8 vp[kStages][P::n], vq[kStages][Q::n];
+  // a tile's r from its first on, and its rows' columns, as they are stored
+  const int64_t left0 = a.r - (int64_t)first * kR;
+  const int64_t p_columns = p.columns, q_columns = q.columns;
+  int loaded = 0;
+  auto load = [&](int set) {          // the next tile, the last one for ever
+    const int64_t left = left0 - (int64_t)loaded * kR;
+    p.load(vp[set], a.p_stride, left);
+    q.load(vq[set], a.q_stride, left);
+    if (loaded + 1 < count) {
+      ++loaded;
+      p.next(a.p_stride);
+      q.next(a.q_stride);
     }
+  };
+  auto store = [&](int set, int t) {
+    const int64_t done = (int64_t)t * kR;
+    p.store(vp[set], lds + set * kBytes, left0 - done, p_columns - done, edge_p);
+    q.store(vq[set], lds + set * kBytes + kPBytes, left0 - done, q_columns - done, edge_q);
+  };
+  using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
+  F one, two;
 #pragma unroll
-    for (int k = 0; k < kR; k += 32) {
-      s16x8 fp[FI], fq[FJ];
-#pragma unroll
-      for (int x = 0; x < FI; ++x) fp[x] = P::fragment(lds, wi + x * 16, k);
-#pragma unroll
-      for (int y = 0; y < FJ; ++y)
-        fq[y] = Q::fragment(lds + P::bytes, wj + y * 16, k);
-#pragma unroll
-      for (int x = 0; x < FI; ++x)
-#pragma unroll
-        for (int y = 0; y < FJ; ++y)
-          acc[x][y] = mma(fq[y], fp[x], acc[x][y], T());
-    }
-  }
+  for (int k = 0; k < kStages; ++k) load(k);
+  store(0, 0);
+  load(0);
+  store(1, 1);
+  load(1);
   __syncthreads();
-  put<T, FI, FJ, 1, EPI>(a, acc, lds + wave * put_bytes<FJ, 1>(), at.split, i0 + wi, j0 + wj);
+  one.read(lds, wi, wj);
+  // the tile t % 4 == k
+  auto step = [&](int t, int k, const F& now, F& next) {
+    __syncthreads();
+    store((k + 2) & 3, t + 2);
+    load((k + 2) & 3);
+    next.read(lds + ((k + 1) & 3) * kBytes, wi, wj);
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(now.q[y], now.p[x], acc[x][y], T());
+    spread<kReads, P::n + Q::n>();
+  };
+  int t = 0;
+  for (; t + 4 <= count; t += 4) {
+    step(t, 0, one, two);
+    step(t + 1, 1, two, one);
+    step(t + 2, 2, one, two);
+    step(t + 3, 3, two, one);
+  }
+  if (t < count) step(t, 0, one, two);
+  if (t + 1 < count) step(t + 1, 1, two, one);
+  if (t + 2 < count) step(t + 2, 2, one, two);
+  __syncthreads();
+  static_assert(WI * WJ * put_bytes<FJ, 2>() <= sizeof(lds), "LDS");
+  put<T, FI, FJ, 2, EPI>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi,
+                         j0 + wj);
 }
 
 // ---- whole chunks: straight from memory into LDS
@@ -404,7 +509,7 @@ __device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
 // there. Chunks behind r's end come from a block of zeros.
 template <typename T, int B, bool TR, int NT>
 struct Direct {
-  using L = Tile<B, TR, kDR>;
+  using L = Tile<B, TR>;
   static constexpr int n = L::rows * L::chunks / NT;
   const T* tile;              // the same for all lanes; moves on with each tile
   uint32_t offset[n];         // bytes from there; stays
@@ -431,7 +536,7 @@ struct Direct {
   // left: how many r there are from the tile's first on
   __device__ __forceinline__ void load(uint32_t lds, int64_t stride, int64_t left) {
     lds += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-    if (left >= kDR) {
+    if (left >= kR) {
 #pragma unroll
       for (int k = 0; k < n; ++k) to_lds(tile, offset[k], lds + k * NT * 16);
     } else {
@@ -444,34 +549,9 @@ struct Direct {
         to_lds(p, lds + k * NT * 16);
       }
     }
-    tile += TR ? kDR * stride : kDR;
+    tile += TR ? kR * stride : kR;
   }
 };
-
-// A tile's fragments of a wave.
-template <int BI, int BJ, int FI, int FJ, bool PT, bool QT>
-struct Fragments {
-  s16x8 p[FI], q[FJ];
-  __device__ __forceinline__ void read(const char* lds, int wi, int wj) {
-#pragma unroll
-    for (int x = 0; x < FI; ++x)
-      p[x] = Tile<BI, PT, kDR>::fragment(lds, wi + x * 16, 0);
-#pragma unroll
-    for (int y = 0; y < FJ; ++y)
-      q[y] = Tile<BJ, QT, kDR>::fragment(lds + Tile<BI, PT, kDR>::bytes, wj + y * 16, 0);
-  }
-};
-
-// Asks the scheduler to spread READS LDS reads over MMAS matrix instructions.
-template <int READS, int MMAS>
-__device__ __forceinline__ void spread() {
-  constexpr int each = MMAS / READS > 0 ? MMAS / READS : 1;
-#pragma unroll
-  for (int i = 0; i < READS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
-    __builtin_amdgcn_sched_group_barrier(0x008, each, 0);   // matrix instructions
-  }
-}
 
 // Four tiles of LDS under way and two sets of fragments, one multiplied while the
 // other is read. A step's barrier says that the next tile has arrived, and that
@@ -484,8 +564,8 @@ void product_direct_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
-  constexpr int kPBytes = Tile<BI, PT, kDR>::bytes;
-  constexpr int kBytes = kPBytes + Tile<BJ, QT, kDR>::bytes;
+  constexpr int kPBytes = Tile<BI, PT>::bytes;
+  constexpr int kBytes = kPBytes + Tile<BJ, QT>::bytes;
   constexpr int kLoads = Direct<T, BI, PT, NT>::n + Direct<T, BJ, QT, NT>::n;
   // s_waitcnt: at most two tiles' loads under way, no LDS read
   constexpr int kLeave = 2 * kLoads;
@@ -496,7 +576,7 @@ void product_direct_kernel(Product a, Tiles map) {
   const Place at = map.place(blockIdx.x);
   const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
-  const int tiles = (int)((a.r + kDR - 1) / kDR);
+  const int tiles = (int)((a.r + kR - 1) / kR);
   const int first = (int)((int64_t)tiles * at.split / a.splits);
   const int count = (int)((int64_t)tiles * (at.split + 1) / a.splits) - first;
   f32x4 acc[FI][FJ];
@@ -506,17 +586,17 @@ void product_direct_kernel(Product a, Tiles map) {
     for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
   Direct<T, BI, PT, NT> p;
   Direct<T, BJ, QT, NT> q;
-  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kDR);
-  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kDR);
-  int64_t left = a.r - (int64_t)first * kDR;
-  const int64_t over = left - (int64_t)count * kDR;      // another block's
+  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kR);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kR);
+  int64_t left = a.r - (int64_t)first * kR;
+  const int64_t over = left - (int64_t)count * kR;      // another block's
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   int stage = 0;                                         // the next load's
   auto load = [&]() {
     const int64_t mine = left - (over > 0 ? over : 0);
     p.load(lds0 + stage, a.p_stride, mine);
     q.load(lds0 + stage + kPBytes, a.q_stride, mine);
-    left -= kDR;
+    left -= kR;
     stage = stage == (kStages - 1) * kBytes ? 0 : stage + kBytes;
   };
   using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
@@ -531,7 +611,7 @@ void product_direct_kernel(Product a, Tiles map) {
     for (int x = 0; x < FI; ++x)
 #pragma unroll
       for (int y = 0; y < FJ; ++y) acc[x][y] = mma(now.q[y], now.p[x], acc[x][y], T());
-    spread<kReads, FI * FJ>();
+    spread<kReads>();
   };
   F one, two;
 #pragma unroll 1
