@@ -447,13 +447,29 @@ Rows product_rows_of(const Tensor& in) {
   return r;
 }
 
+bool chunked(const Rows& r) {
+  return r.t.size(-1) % 8 == 0 && r.stride % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0;
+}
+
+// A weight's rows as whole aligned chunks of 8, with zeros behind them: a copy
+// where they are not, so that the other operand alone decides how loads go.
+Rows weight_rows_of(const Tensor& in) {
+  const Rows r = product_rows_of(in);
+  if (chunked(r)) return r;
+  const Tensor wide = torch::constant_pad_nd(in, {0, (8 - in.size(-1) % 8) % 8}, 0).contiguous();
+  return {wide, r.rows, wide.size(-1)};
+}
+
 void run_product(blk::Product& a, int dtype, const Tensor& like) {
   TORCH_CHECK_VALUE(a.i < (int64_t)1 << 32 && a.r < (int64_t)1 << 32,
                     "more than 2^32 rows");
   a.splits = blk::product_splits(a);
   Tensor partial;
   if (a.splits > 1) {
-    partial = torch::empty({a.splits, a.i, a.j}, like.options().dtype(torch::kFloat32));
+    a.partial_cols = (a.j + 7) / 8 * 8;
+    partial = torch::empty({a.splits, a.i, a.partial_cols},
+                           like.options().dtype(torch::kFloat32));
     a.partial = partial.data_ptr<float>();
   }
   blk::product(a, dtype, stream_of(like));
@@ -491,7 +507,9 @@ std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
                       "residual must be of the output's shape");
   }
   const c10::DeviceGuard guard(x.device());
-  const Rows xr = product_rows_of(x), wr = product_rows_of(weight.to(x.scalar_type()));
+  const Rows xr = product_rows_of(x);
+  const Tensor w = weight.to(x.scalar_type());
+  const Rows wr = chunked(xr) ? weight_rows_of(w) : product_rows_of(w);
   if (bias.has_value()) bias = bias->contiguous();
   const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
   Tensor y = torch::empty(shape, x.options());
@@ -564,7 +582,8 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
   }
   const Rows zr = need_x || need_w ? product_rows_of(dz) : Rows{dz, 0, 0};
   if (need_x) {
-    const Rows wr = product_rows_of(weight.to(x.scalar_type()));
+    const Tensor w = weight.to(x.scalar_type());
+    const Rows wr = chunked(zr) ? weight_rows_of(w) : product_rows_of(w);
     blk::Product a{};
     a.p = zr.t.data_ptr();
     a.q = wr.t.data_ptr();

@@ -78,8 +78,8 @@ enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
 struct Product {
   const void *p, *q;
   int64_t p_stride, q_stride;
-  int64_t p_cols, q_cols;                     // a row's elements, 8 at least: what
-                                              // lies behind i, j or r is zero
+  int64_t p_cols, q_cols;                     // a row's elements, 8 at least: those
+                                              // behind r are zero
   int64_t i, j, r;
   bool p_t, q_t;
   void *out;                                  // [i][j], contiguous
@@ -91,7 +91,8 @@ struct Product {
   void *z;                                    // what goes into act, or null
   int act;
   int splits;                                 // parts of r ...
-  float *partial;                             // ... [splits][i][j], or null
+  float *partial;                             // ... [splits][i][partial_cols],
+  int64_t partial_cols;                       // j up to a multiple of 8; or null
 };
 struct ActBwd {
   const void *dy, *z;                         // z: or null without act

@@ -385,7 +385,7 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
                                                      lane % kLanes * 8, 16), 32);
         if (i >= a.i || n <= 0) continue;
         if (EPI == kPlain && a.partial)
-          store_some<float, 8>(a.partial + (split * a.i + i) * a.j + j, n, v);
+          store_run<float, 8>(a.partial + (split * a.i + i) * a.partial_cols + j, v);
         else
           finish<T, EPI>(a, i, j, n, v, bias, r[g]);
       }
@@ -513,17 +513,21 @@ struct Direct {
   static constexpr int n = L::rows * L::chunks / NT;
   const T* tile;              // the same for all lanes; moves on with each tile
   uint32_t offset[n];         // bytes from there; stays
+  int64_t ahead;              // r, or a row's elements, from the tile's first on
 
+  // cols: a row's elements in memory, a multiple of 8
   __device__ __forceinline__ void start(const T* base, int64_t stride, int64_t i0,
-                                        int64_t i_end, int64_t r0) {
+                                        int64_t i_end, int64_t r0, int64_t r_end,
+                                        int64_t cols) {
     tile = TR ? base + r0 * stride + i0 : base + i0 * stride + r0;
+    ahead = (TR ? r_end : cols < r_end + 8 ? cols : r_end) - r0;
 #pragma unroll
     for (int k = 0; k < n; ++k) {
       const int slot = k * NT + threadIdx.x;
       const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
       int64_t at;
       if constexpr (TR) {
-        const int64_t last = i_end - 8 - i0;
+        const int64_t last = cols - 8 - i0;
         at = row * stride + (chunk * 8 < last ? chunk * 8 : last);
       } else {
         const int64_t last = i_end - 1 - i0;
@@ -533,10 +537,9 @@ struct Direct {
     }
   }
 
-  // left: how many r there are from the tile's first on
-  __device__ __forceinline__ void load(uint32_t lds, int64_t stride, int64_t left) {
+  __device__ __forceinline__ void load(uint32_t lds, int64_t stride) {
     lds += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-    if (left >= kR) {
+    if (ahead >= kR) {
 #pragma unroll
       for (int k = 0; k < n; ++k) to_lds(tile, offset[k], lds + k * NT * 16);
     } else {
@@ -544,20 +547,21 @@ struct Direct {
       for (int k = 0; k < n; ++k) {
         const int slot = k * NT + threadIdx.x;
         const int row = slot / L::chunks, chunk = L::place(row, slot % L::chunks);
-        const char* p = (TR ? row : chunk * 8) < left ? (const char*)tile + offset[k]
-                                                      : (const char*)kZeros;
+        const char* p = (TR ? row : chunk * 8) < ahead ? (const char*)tile + offset[k]
+                                                       : (const char*)kZeros;
         to_lds(p, lds + k * NT * 16);
       }
     }
     tile += TR ? kR * stride : kR;
+    ahead -= kR;
   }
 };
 
 // Four tiles of LDS under way and two sets of fragments, one multiplied while the
 // other is read. A step's barrier says that the next tile has arrived, and that
 // this one is in registers, so that its LDS can take the tile four further on.
-// Every step loads a tile, zeros behind the last, so that a fixed number of
-// loads is under way and a wait can leave the youngest two tiles' alone.
+// Every step loads a tile, zeros behind r's end, so that a fixed number of loads
+// is under way and a wait can leave the youngest two tiles' alone.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 2)
 void product_direct_kernel(Product a, Tiles map) {
@@ -586,17 +590,14 @@ void product_direct_kernel(Product a, Tiles map) {
     for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
   Direct<T, BI, PT, NT> p;
   Direct<T, BJ, QT, NT> q;
-  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kR);
-  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kR);
-  int64_t left = a.r - (int64_t)first * kR;
-  const int64_t over = left - (int64_t)count * kR;      // another block's
+  // another block's tiles are loaded behind the last one, and not used
+  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kR, a.r, a.p_cols);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kR, a.r, a.q_cols);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   int stage = 0;                                         // the next load's
   auto load = [&]() {
-    const int64_t mine = left - (over > 0 ? over : 0);
-    p.load(lds0 + stage, a.p_stride, mine);
-    q.load(lds0 + stage + kPBytes, a.q_stride, mine);
-    left -= kR;
+    p.load(lds0 + stage, a.p_stride);
+    q.load(lds0 + stage + kPBytes, a.q_stride);
     stage = stage == (kStages - 1) * kBytes ? 0 : stage + kBytes;
   };
   using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
@@ -646,12 +647,12 @@ __global__ __launch_bounds__(256) void product_join_kernel(Product a) {
     load_bias<T>(a, j, n, bias);
     if (a.residual) residual = load_residual<T>(a, i, j, n);
   }
-  const float* p = a.partial + i * a.j + j;
-  const int64_t part = a.i * a.j;
+  const float* p = a.partial + i * a.partial_cols + j;
+  const int64_t part = a.i * a.partial_cols;
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     float q[8];
-    load_some<float, 8>(p + s * part, n, q, 0.f);
+    load_run<float, 8>(p + s * part, q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += q[e];
   }
@@ -730,15 +731,15 @@ __global__ __launch_bounds__(1024) void bias_join_kernel(ActBwd a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-bool chunked(const void* p, int64_t stride, bool t, int64_t i, int64_t r) {
-  // a tile's offsets are 32-bit
+// Whether an operand's rows are whole aligned chunks of 8, and a tile's offsets
+// fit 32 bits.
+bool chunked(const void* p, int64_t stride, int64_t cols) {
   return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && stride < (1 << 22) &&
-         (t ? i : r) % 8 == 0;
+         cols % 8 == 0;
 }
 
 bool direct(const Product& a) {
-  return chunked(a.p, a.p_stride, a.p_t, a.i, a.r) &&
-         chunked(a.q, a.q_stride, a.q_t, a.j, a.r);
+  return chunked(a.p, a.p_stride, a.p_cols) && chunked(a.q, a.q_stride, a.q_cols);
 }
 
 bool large(const Product& a) {
