@@ -659,6 +659,84 @@ __global__ __launch_bounds__(256) void product_join_kernel(Product a) {
   finish<T, EPI>(a, i, j, n, v, bias, residual);
 }
 
+// ---- few rows
+
+constexpr int kFewRows = 64;
+constexpr int kFewWaves = 8;
+
+// 16 columns of the output for at most MT x 16 rows: what bounds a layer with few
+// rows is how soon its weights arrive, so each of 8 waves asks for an eighth of r
+// of both operands straight into fragments, and the waves' sums meet in LDS. One
+// launch, and no parts to join: 16 x 1024 by 256 takes 4.8 us, by tiles of 128
+// with r in parts 8.9 us.
+template <typename T, int MT, int EPI>
+__global__ __launch_bounds__(kFewWaves * 64)
+void product_few_kernel(Product a) {
+  __shared__ __attribute__((aligned(16))) float part[kFewWaves][MT * 16][16];
+  constexpr int kAhead = MT > 2 ? 2 : 4;      // steps of 32 r under way together
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t j0 = (int64_t)blockIdx.x * 16;
+  const int64_t j = j0 + (lane & 15) < a.j ? j0 + (lane & 15) : a.j - 1;
+  const T* q = (const T*)a.q + j * a.q_stride;
+  const T* p[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int64_t i = m * 16 + (lane & 15);
+    p[m] = (const T*)a.p + (i < a.i ? i : a.i - 1) * a.p_stride;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = (f32x4)0.f;
+  const int chunk = (lane >> 4) * 8;
+  // 8 elements from r on; the last ones of a row by way of those before them
+  auto load = [&](const T* row, int64_t r, int64_t cols) {
+    s16x8 v;
+    const int64_t at = r < cols - 8 ? r : cols - 8;
+    __builtin_memcpy(&v, row + at, 16);
+    return v;
+  };
+  auto placed = [&](s16x8 v, int64_t r, int64_t cols) {
+    const int64_t by = r - (cols - 8);
+    return by > 0 ? Staged<T, 128, false, 256>::moved(v, by < 8 ? (int)by : 8) : v;
+  };
+  for (int64_t r0 = wave * 32; r0 < a.r; r0 += kFewWaves * 32 * kAhead) {
+    s16x8 fq[kAhead], fp[kAhead][MT];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t r = r0 + k * kFewWaves * 32 + chunk;
+      fq[k] = load(q, r, a.q_cols);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) fp[k][m] = load(p[m], r, a.p_cols);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t r = r0 + k * kFewWaves * 32 + chunk;
+      fq[k] = placed(fq[k], r, a.q_cols);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        acc[m] = mma(fq[k], placed(fp[k][m], r, a.p_cols), acc[m], T());
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    *(f32x4*)&part[wave][m * 16 + (lane & 15)][(lane >> 4) * 4] = acc[m];
+  __syncthreads();
+  const int64_t i = threadIdx.x >> 1, at = j0 + (threadIdx.x & 1) * 8;
+  if (i >= a.i || at >= a.j || i >= MT * 16) return;
+  const int n = a.j - at < 8 ? (int)(a.j - at) : 8;
+  float bias[8], v[8] = {};
+  s16x8 residual = (s16x8)0;
+  if constexpr (EPI != kPlain) {
+    load_bias<T>(a, at, n, bias);
+    if (a.residual) residual = load_residual<T>(a, i, at, n);
+  }
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += part[w][i][(threadIdx.x & 1) * 8 + e];
+  finish<T, EPI>(a, i, at, n, v, bias, residual);
+}
+
 // ---- dz and db
 
 constexpr int kActRows = 4;           // rows of a thread under way together
@@ -742,12 +820,29 @@ bool direct(const Product& a) {
   return chunked(a.p, a.p_stride, a.p_cols) && chunked(a.q, a.q_stride, a.q_cols);
 }
 
+bool few(const Product& a) { return a.i <= kFewRows && !a.p_t && !a.q_t; }
+
+// Tiles of 256 x 256, of which one fills a compute unit, need 1024 r to outweigh
+// their first loads and their output (32768 x 1000 by 256 takes 34 us by tiles of
+// 128, 52 us by these), and either enough of them for all compute units or enough
+// r to share a tile among two blocks (with 128 tiles of only 1024 r, 2048 x 1024 by
+// 4096 takes 49 us in two parts, 29 us by tiles of 128).
 bool large(const Product& a) {
-  return direct(a) && ceil_div(a.i, 256) * ceil_div(a.j, 256) >= 100;
+  const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
+  return direct(a) && ((a.r >= 1024 && tiles >= 192) || (a.r >= 4096 && tiles >= 96));
 }
 
 template <typename T, bool PT, bool QT, int EPI>
 void launch(const Product& a, hipStream_t stream) {
+  if constexpr (!PT && !QT) {
+    if (few(a)) {
+      const dim3 grid((unsigned)ceil_div(a.j, 16));
+      if (a.i <= 16) product_few_kernel<T, 1, EPI><<<grid, kFewWaves * 64, 0, stream>>>(a);
+      else if (a.i <= 32) product_few_kernel<T, 2, EPI><<<grid, kFewWaves * 64, 0, stream>>>(a);
+      else product_few_kernel<T, 4, EPI><<<grid, kFewWaves * 64, 0, stream>>>(a);
+      return;
+    }
+  }
   const int side = large(a) ? 256 : 128;
   const Tiles map = {(int)ceil_div(a.i, side), (int)ceil_div(a.j, side), a.splits};
   const dim3 grid((unsigned)map.i * map.j * map.splits);
@@ -802,6 +897,7 @@ void launch_act_bwd(const ActBwd& a, hipStream_t stream) {
 }  // namespace
 
 int product_splits(const Product& a) {
+  if (few(a)) return 1;
   if (large(a)) {
     const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
     return tiles <= 128 ? 2 : 1;
