@@ -32,6 +32,9 @@ class ReinforcementLoss:
         self.kl_head_weights = self.cfg.kl_head_weights
         self.only_update_value = False
         self.use_total_rhos = self.cfg.get('use_total_rhos', False)
+        # log-probs and entropy of a head in one pass over its logits, in their
+        # own type (ops/token_logprobs.py), instead of one float32 pass each
+        self.fused_logprobs = self.cfg.get('fused_logprobs', False)
 
     def compute_loss(self, inputs):
         target_logits_dict = inputs['target_logit']        # (T, B, ...)
@@ -68,9 +71,17 @@ class ReinforcementLoss:
             target_logits = target_logits_dict[head_type]
             actions = actions_dict[head_type]
             num_classes_dict[head_type] = target_logits.shape[-1]
-            target_action_log_probs = -masked_cross_entropy(target_logits,
-                                                            actions)
-            entropy_rows_dict[head_type] = rowwise_entropy(target_logits)
+            if self.fused_logprobs:
+                from ..ops.token_logprobs import token_logprobs
+                if head_type == 'selected_units':
+                    actions = actions.masked_fill(~masks_dict['selected_units_mask'], -100)
+                got = token_logprobs(target_logits, actions, ignore_index=-100)
+                target_action_log_probs = got.logprob
+                entropy_rows_dict[head_type] = got.entropy
+            else:
+                target_action_log_probs = -masked_cross_entropy(target_logits,
+                                                                actions)
+                entropy_rows_dict[head_type] = rowwise_entropy(target_logits)
             kl_rows_dict[head_type] = rowwise_kl(
                 teacher_logits_dict[head_type], target_logits)
             if self.use_dapo:

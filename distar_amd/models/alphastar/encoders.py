@@ -47,7 +47,8 @@ class BeginningBuildOrderEncoder(nn.Module):
         self.act = build_activation(self.cfg.activation)
         self.transformer = Transformer(
             input_dim=self.input_dim, head_dim=self.cfg.head_dim,
-            hidden_dim=self.cfg.output_dim * 2, output_dim=self.cfg.output_dim)
+            hidden_dim=self.cfg.output_dim * 2, output_dim=self.cfg.output_dim,
+            fused=self.cfg.get('fused', False))
         self.embedd_fc = fc_block(self.cfg.output_dim, self.output_dim, activation=self.act)
         self.action_one_hot = one_hot_embedding(self.cfg.action_one_hot_dim)
         self.order_one_hot = one_hot_embedding(20)
@@ -255,7 +256,8 @@ class EntityEncoder(nn.Module):
             hidden_dim=self.cfg.hidden_dim, output_dim=self.cfg.output_dim,
             head_num=self.cfg.head_num, mlp_num=self.cfg.mlp_num,
             layer_num=self.cfg.layer_num, dropout_ratio=self.cfg.dropout_ratio,
-            activation=self.act, ln_type=self.cfg.ln_type)
+            activation=self.act, ln_type=self.cfg.ln_type,
+            fused=self.cfg.get('fused', False))
         self.entity_fc = fc_block(self.cfg.output_dim, self.cfg.output_dim, activation=self.act)
         self.embed_fc = fc_block(self.cfg.output_dim, self.cfg.output_dim, activation=self.act)
         reduce_type = self.whole_cfg.model.entity_reduce_type

@@ -72,7 +72,9 @@ class Model(nn.Module):
 
     # ------------------------------------------------------ actor inference
     def compute_logp_action(self, spatial_info, entity_info, scalar_info,
-                            entity_num, hidden_state, **kwargs):
+                            entity_num, hidden_state, top_k=0, **kwargs):
+        """With `top_k`, also each head's likeliest actions and their log
+        probabilities, as ``action_alternatives[head] = (actions, logp)``."""
         lstm_input, scalar_context, baseline_feature, entity_embeddings, map_skip = \
             self.encoder(spatial_info, entity_info, scalar_info, entity_num)
         lstm_output, out_state = self.core_lstm(lstm_input.unsqueeze(0), hidden_state)
@@ -82,9 +84,16 @@ class Model(nn.Module):
         for k, action in action_info.items():
             dist = torch.distributions.Categorical(logits=logit[k])
             log_action_probs[k] = dist.log_prob(action)
-        return {'action_info': action_info, 'action_logp': log_action_probs,
-                'selected_units_num': selected_units_num, 'entity_num': entity_num,
-                'hidden_state': out_state, 'logit': logit, 'extra_units': extra_units}
+        out = {'action_info': action_info, 'action_logp': log_action_probs,
+               'selected_units_num': selected_units_num, 'entity_num': entity_num,
+               'hidden_state': out_state, 'logit': logit, 'extra_units': extra_units}
+        if top_k:
+            from ...ops.token_logprobs import token_logprobs
+            out['action_alternatives'] = {}
+            for k, action in action_info.items():
+                got = token_logprobs(logit[k], action, top_k=top_k)
+                out['action_alternatives'][k] = (got.top_tokens, got.top_logprobs)
+        return out
 
     # ------------------------------------------------------- teacher logits
     def compute_teacher_logit(self, spatial_info, entity_info, scalar_info,

@@ -57,6 +57,9 @@ def build_normalization(norm_type, dim=None):
     if norm_type is None or norm_type == 'none':
         return None
     key = norm_type if dim is None else f'{norm_type}{dim}D'
+    if key in ('FusedLN', 'FusedLN1D'):
+        from ...ops.layer_norm import FusedLayerNorm
+        return FusedLayerNorm
     norms = {
         'BN': nn.BatchNorm1d, 'BN1D': nn.BatchNorm1d, 'BN2D': nn.BatchNorm2d,
         'LN': nn.LayerNorm, 'LN1D': nn.LayerNorm, 'LN2D': nn.LayerNorm,

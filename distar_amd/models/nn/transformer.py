@@ -35,6 +35,10 @@ class Attention(nn.Module):
     def forward(self, x, mask: Optional[torch.Tensor] = None):
         """`mask`: (B, N) boolean key-validity PREFIX mask (sequence_mask of
         the entity count) or None."""
+        return self.project(self.core(x, mask))
+
+    def core(self, x, mask: Optional[torch.Tensor] = None):
+        """The heads' outputs side by side, before the projection."""
         assert len(x.shape) == 3
         B, N = x.shape[:2]
         qkv = self.attention_pre(x)                      # (B, N, 3*H*D)
@@ -45,9 +49,8 @@ class Attention(nn.Module):
         if use_hip:
             from ...ops.entity_attn import entity_attention
             entity_num = mask.int().sum(dim=-1) if mask is not None else None
-            attention = entity_attention(qkv, entity_num, self.head_num,
-                                         1.0 / math.sqrt(self.head_dim))
-            return self.project(attention)
+            return entity_attention(qkv, entity_num, self.head_num,
+                                    1.0 / math.sqrt(self.head_dim))
         qkv = qkv.view(B, N, 3, self.head_num, self.head_dim)
         qkv = qkv.permute(2, 0, 3, 1, 4)  # 3, B, H, N, D
         query, key, value = qkv[0], qkv[1], qkv[2]
@@ -74,14 +77,19 @@ class Attention(nn.Module):
             if self.dropout is not None:
                 score = self.dropout(score)
             attention = torch.matmul(score, value)                   # B, H, N, D
-        attention = attention.permute(0, 2, 1, 3).reshape(B, N, -1)  # B, N, H*D
-        return self.project(attention)
+        return attention.permute(0, 2, 1, 3).reshape(B, N, -1)       # B, N, H*D
 
 
 class TransformerLayer(nn.Module):
+    """`fused`: a pre-norm layer without dropout on the block operators (same
+    state dict): `ops/layer_norm.py` for the norms, `ops/linear_act.py` for the
+    projection and the MLP, whose epilogues add the residual stream.  On a GPU
+    it needs autocast to bfloat16 or float16, the stream's type then."""
+
     def __init__(self, input_dim, head_dim, hidden_dim, output_dim, head_num,
-                 mlp_num, dropout, activation, ln_type):
+                 mlp_num, dropout, activation, ln_type, fused=False):
         super().__init__()
+        self.fused = fused
         self.attention = Attention(input_dim, head_dim, output_dim, head_num, dropout)
         self.layernorm1 = build_normalization('LN')(output_dim)
         self.dropout = dropout
@@ -94,9 +102,35 @@ class TransformerLayer(nn.Module):
         self.mlp = nn.Sequential(*layers)
         self.layernorm2 = build_normalization('LN')(output_dim)
         self.ln_type = ln_type
+        if fused:
+            self._fuse(dims, activation)
+
+    def _fuse(self, dims, activation):
+        from ...ops.linear_act import LinearAct
+        act = {nn.ReLU: 'relu', nn.GELU: 'gelu', nn.SiLU: 'silu',
+               type(None): None}.get(type(activation), '?')
+        if self.ln_type != 'pre' or self.dropout is not None or act == '?':
+            raise ValueError('fused layers are pre-norm, without dropout, and have a relu, '
+                             f'gelu or silu; got {self.ln_type}, {self.dropout}, {activation}')
+
+        def fused(linear, act):
+            new = LinearAct(linear.in_features, linear.out_features, activation=act)
+            new.weight, new.bias = linear.weight, linear.bias
+            return nn.Sequential(new)
+
+        self.attention.project = fused(self.attention.project[0], None)
+        self.mlp = nn.Sequential(*[fused(block[0], act) for block in self.mlp])
+        for name in ('layernorm1', 'layernorm2'):
+            setattr(self, name, build_normalization('FusedLN')(dims[-1]))
 
     def forward(self, x, mask: Optional[torch.Tensor] = None):
-        if self.ln_type == 'post':
+        if self.fused:
+            x = self.attention.project[0](self.attention.core(self.layernorm1(x), mask), x)
+            m = self.layernorm2(x)
+            for block in self.mlp[:-1]:
+                m = block(m)
+            x = self.mlp[-1][0](m, x)
+        elif self.ln_type == 'post':
             a = self.attention(x, mask)
             if self.dropout is not None:
                 a = self.dropout(a)
@@ -123,14 +157,14 @@ class TransformerLayer(nn.Module):
 class Transformer(nn.Module):
     def __init__(self, input_dim, head_dim=128, hidden_dim=1024, output_dim=256,
                  head_num=2, mlp_num=2, layer_num=3, dropout_ratio=0.0,
-                 activation=nn.ReLU(), ln_type='pre'):
+                 activation=nn.ReLU(), ln_type='pre', fused=False):
         super().__init__()
         self.embedding = fc_block(input_dim, output_dim, activation=activation)
         self.act = activation
         self.dropout = nn.Dropout(dropout_ratio) if dropout_ratio > 0 else None
         self.layers = nn.ModuleList([
             TransformerLayer(output_dim, head_dim, hidden_dim, output_dim,
-                             head_num, mlp_num, self.dropout, self.act, ln_type)
+                             head_num, mlp_num, self.dropout, self.act, ln_type, fused)
             for _ in range(layer_num)
         ])
 

@@ -734,3 +734,100 @@ def test_second_derivatives_are_refused_and_versions_kept(device):
     clip_grad_norm([b], 0.1)
     with pytest.raises(RuntimeError):
         y.backward()
+
+
+# ------------------------------------------------------------------ in the framework
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_transformer_on_block_operators(device):
+    from distar_amd.models.nn.transformer import Transformer
+    torch.manual_seed(0)
+    args = dict(input_dim=48, head_dim=128, hidden_dim=160, output_dim=96, head_num=2, layer_num=2)
+    plain, fused = Transformer(**args).to(device), Transformer(**args, fused=True).to(device)
+    fused.load_state_dict(plain.state_dict())
+    assert list(plain.state_dict()) == list(fused.state_dict())
+    x = torch.randn(3, 20, 48, device=device)
+    mask = torch.arange(20, device=device) < torch.tensor([[20], [7], [1]], device=device)
+    dy = torch.randn(3, 20, 96, device=device)
+    want = plain(x, mask)
+    ref = torch.autograd.grad(want, list(plain.parameters()), dy)
+    if device == 'cpu':
+        got = fused(x, mask)
+        off = 1e-5
+    else:
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            got = fused(x, mask)
+        assert got.dtype == torch.bfloat16
+        off = 16 * half(torch.bfloat16)       # some twenty stored values on the way
+    grads = torch.autograd.grad(got, list(fused.parameters()), dy.to(got.dtype))
+    # A relu's input carries the noise n of about four stored values, 4 half steps of
+    # its own size; of normal values the share 0.8 n lies that near to zero, and each of
+    # those may change sides, which takes its whole gradient along: a relative error of
+    # sqrt(0.8 n) for one relu, and of sqrt(5 * 0.8 n) for the five of this model.
+    flips = math.sqrt(5 * 0.8 * 4 * half(got.dtype)) if device == 'cuda' else 0.
+    for a, b, most in zip([got, *grads], [want, *ref], [off] + [off + flips] * len(grads)):
+        a, b = a.double(), b.double()
+        assert torch.linalg.vector_norm(a - b) <= most * torch.linalg.vector_norm(b) + 1e-6
+    with pytest.raises(ValueError):
+        Transformer(**args, fused=True, ln_type='post')
+    with pytest.raises(ValueError):
+        Transformer(**args, fused=True, dropout_ratio=0.1)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_rl_loss_with_fused_logprobs(device):
+    from distar_amd.lib.fake_data import fake_rl_learner_data
+    from distar_amd.losses import ReinforcementLoss
+    from distar_amd.models import Model
+    from distar_amd.utils.config import Config
+    from distar_amd.utils.data import to_device
+    torch.manual_seed(0)
+    model = Model(Config({'common': {'type': 'train'}, 'model': {'enable_baselines': ['winloss']}}),
+                  use_value_network=True).to(device)
+    data = fake_rl_learner_data(batch_size=2, unroll_len=3, entity_num_range=(32, 48))
+    for key in ('model_last_iter', 'aux_type'):
+        data.pop(key)
+    out = model.rl_learner_forward(**to_device(data, device))
+    total, grads = [], []
+    for fused in (False, True):
+        loss = ReinforcementLoss(Config({'fused_logprobs': fused}), 'MP0')
+        assert loss.fused_logprobs is fused
+        leaves = {k: v.detach().requires_grad_() for k, v in out['target_logit'].items()}
+        values = {k: v.detach().clone() for k, v in out['value'].items()}
+        total.append(loss.compute_loss({**out, 'target_logit': leaves, 'value': values})['total_loss'])
+        grads.append(torch.autograd.grad(total[-1], list(leaves.values())))
+    # the same quantities in 32 bits by two ways
+    torch.testing.assert_close(total[0], total[1], rtol=1e-4, atol=1e-5)
+    for a, b in zip(*grads):
+        assert torch.linalg.vector_norm(a - b) <= 1e-4 * torch.linalg.vector_norm(a) + 1e-7
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_inference_alternatives_and_fused_norm_blocks(device):
+    from distar_amd.lib.fake_data import fake_sl_batch
+    from distar_amd.models import Model
+    from distar_amd.models.nn.blocks import ResFCBlock2, build_normalization
+    from distar_amd.utils.config import Config
+    from distar_amd.utils.data import to_device
+    torch.manual_seed(0)
+    model = Model(Config({'common': {'type': 'train'}})).to(device)
+    data = to_device(fake_sl_batch(batch_size=2, traj_len=1, entity_num=32), device)
+    hidden = [(torch.zeros(2, 384, device=device), torch.zeros(2, 384, device=device)) for _ in range(3)]
+    obs = {k: data[k] for k in ('spatial_info', 'entity_info', 'scalar_info', 'entity_num')}
+    with torch.no_grad():
+        out = model.compute_logp_action(**obs, hidden_state=hidden, top_k=4)
+    for head, (tokens, logp) in out['action_alternatives'].items():
+        logit = out['logit'][head]
+        k = min(4, logit.shape[-1])
+        assert tokens.shape == (*logit.shape[:-1], k)
+        best, where = logit.max(-1)
+        assert torch.equal(logit.gather(-1, tokens[..., :1]).squeeze(-1), best)
+        want = torch.log_softmax(logit.double(), -1).gather(-1, tokens.clamp(min=0))
+        torch.testing.assert_close(logp.double(), want, rtol=1e-5, atol=1e-4)
+    with torch.no_grad():
+        assert 'action_alternatives' not in model.compute_logp_action(**obs, hidden_state=hidden)
+    plain, fused = ResFCBlock2(24, norm_type='LN').to(device), ResFCBlock2(24, norm_type='FusedLN').to(device)
+    fused.load_state_dict(plain.state_dict())
+    x = torch.randn(5, 24, device=device)
+    torch.testing.assert_close(fused(x), plain(x), rtol=1e-5, atol=1e-5)
+    assert build_normalization('FusedLN', dim=1) is FusedLayerNorm
