@@ -327,6 +327,7 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(LayerNormBwd a) {
   const int64_t cols = 2 * (int64_t)a.width;
   float v = 0.f;
   if (c < cols)
+#pragma unroll 4
     for (int k = group; k < a.blocks; k += 64) v += a.partial[k * cols + c];
   lds[group][lane] = v;
   __syncthreads();

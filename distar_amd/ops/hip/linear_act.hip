@@ -340,7 +340,7 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
   constexpr int kPitch = FJ * 16 + 4;        // floats; 16 rows meet no bank twice
   constexpr int kLanes = FJ * 2;             // a row's
   constexpr int kRows = 64 / kLanes;         // that a wave takes at once
-  constexpr int kGroup = XP * 16 / kRows < 4 ? XP * 16 / kRows : 4;
+  constexpr int kGroup = XP * 16 / kRows < 8 ? XP * 16 / kRows : 8;
   const int lane = threadIdx.x & 63;
   float* const part = (float*)lds;
   const int64_t j = j0 + lane % kLanes * 8;
@@ -557,25 +557,28 @@ struct Direct {
   }
 };
 
-// Four tiles of LDS under way and two sets of fragments, one multiplied while the
+// S tiles of LDS under way and two sets of fragments, one multiplied while the
 // other is read. A step's barrier says that the next tile has arrived, and that
-// this one is in registers, so that its LDS can take the tile four further on.
-// Every step loads a tile, zeros behind r's end, so that a fixed number of loads
-// is under way and a wait can leave the youngest two tiles' alone.
+// this one is in registers, so that its LDS can take the tile S further on. Every
+// step loads a tile, zeros behind r's end, so that a fixed number of loads is under
+// way and a wait can leave the youngest S - 2 tiles' alone. 256 x 256 takes four
+// tiles and a compute unit, 128 x 128 three, so that three blocks share one.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
-__global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 2)
+__global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 3)
 void product_direct_kernel(Product a, Tiles map) {
+  constexpr int S = BI * BJ > 128 * 128 ? 4 : 3;
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
   constexpr int kPBytes = Tile<BI, PT>::bytes;
   constexpr int kBytes = kPBytes + Tile<BJ, QT>::bytes;
   constexpr int kLoads = Direct<T, BI, PT, NT>::n + Direct<T, BJ, QT, NT>::n;
-  // s_waitcnt: at most two tiles' loads under way, no LDS read
-  constexpr int kLeave = 2 * kLoads;
+  // s_waitcnt: at most S - 2 tiles' loads under way, no LDS read
+  constexpr int kLeave = (S - 2) * kLoads, kFirst = (S - 1) * kLoads;
   constexpr int kWait = (kLeave & 15) | (kLeave >> 4) << 14 | 7 << 4;
-  static_assert(kStages == 4 && kLeave < 64, "waits");
-  __shared__ __attribute__((aligned(16))) char lds[kStages * kBytes];
+  constexpr int kWaitFirst = (kFirst & 15) | (kFirst >> 4) << 14 | 7 << 4;
+  static_assert(kFirst < 64, "waits");
+  __shared__ __attribute__((aligned(16))) char lds[S * kBytes];
   const int wave = threadIdx.x >> 6;
   const Place at = map.place(blockIdx.x);
   const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
@@ -598,7 +601,7 @@ void product_direct_kernel(Product a, Tiles map) {
   auto load = [&]() {
     p.load(lds0 + stage, a.p_stride);
     q.load(lds0 + stage + kPBytes, a.q_stride);
-    stage = stage == (kStages - 1) * kBytes ? 0 : stage + kBytes;
+    stage = stage == (S - 1) * kBytes ? 0 : stage + kBytes;
   };
   using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
   int ready = kBytes;                                    // the tile to read next
@@ -607,7 +610,7 @@ void product_direct_kernel(Product a, Tiles map) {
     __syncthreads();
     load();
     next.read(lds + ready, wi, wj);
-    ready = ready == (kStages - 1) * kBytes ? 0 : ready + kBytes;
+    ready = ready == (S - 1) * kBytes ? 0 : ready + kBytes;
 #pragma unroll
     for (int x = 0; x < FI; ++x)
 #pragma unroll
@@ -616,9 +619,8 @@ void product_direct_kernel(Product a, Tiles map) {
   };
   F one, two;
 #pragma unroll 1
-  for (int k = 0; k < kStages; ++k) load();
-  // the first of the four; the loop's wait counts from three under way
-  __builtin_amdgcn_s_waitcnt((3 * kLoads & 15) | (3 * kLoads >> 4) << 14 | 7 << 4);
+  for (int k = 0; k < S; ++k) load();
+  __builtin_amdgcn_s_waitcnt(kWaitFirst);
   __syncthreads();
   one.read(lds, wi, wj);
   int t = 0;
