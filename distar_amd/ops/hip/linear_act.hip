@@ -19,8 +19,8 @@
 namespace blk {
 namespace {
 
-constexpr int kR = 32;            // r a tile
-constexpr int kStages = 4;        // tiles in LDS
+constexpr int kR = 32;            // r a tile, straight into LDS
+constexpr int kSR = 64;           // r a tile, by way of registers
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -138,13 +138,13 @@ __device__ __forceinline__ s16x8 load_residual(const Product& a, int64_t i, int6
 
 // ---- tiles
 
-// An operand's tile of B i by 32 r in LDS: rows of chunks of 8 elements. With r
-// contiguous a row is one i and holds 32 r; otherwise a row is one r and holds
+// An operand's tile of B i by KR r in LDS: rows of chunks of 8 elements. With r
+// contiguous a row is one i and holds KR r; otherwise a row is one r and holds
 // the tile's B values of i.
-template <int B, bool TR>
+template <int B, bool TR, int KR>
 struct Tile {
-  static constexpr int rows = TR ? kR : B;
-  static constexpr int chunks = TR ? B / 8 : kR / 8;
+  static constexpr int rows = TR ? KR : B;
+  static constexpr int chunks = TR ? B / 8 : KR / 8;
   static constexpr int bytes = rows * chunks * 16;
 
   // The chunk's place in its row. A read with r contiguous takes 16 lanes' rows
@@ -152,11 +152,12 @@ struct Tile {
   // a turning read takes 32 bytes, so there pairs of chunks move together.
   static __device__ __forceinline__ int place(int row, int chunk) {
     if constexpr (TR) return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
-    else return chunk ^ (-(row >> 2) & 3);
+    else if constexpr (KR == 32) return chunk ^ (-(row >> 2) & 3);
+    else return chunk ^ ((row >> 1) & 7);
   }
 
-  // 8 consecutive r from 8 (lane / 16) on of i = i0 + lane % 16
-  static __device__ __forceinline__ s16x8 fragment(const char* lds, int i0) {
+  // 8 consecutive r from r0 + 8 (lane / 16) on of i = i0 + lane % 16
+  static __device__ __forceinline__ s16x8 fragment(const char* lds, int i0, int r0) {
     const int lane = threadIdx.x & 63;
     if constexpr (TR) {
       // lanes 4q ... 4q + 3 of 16 fetch row q's 16 elements; lane c gets
@@ -164,7 +165,7 @@ struct Tile {
       s16x4 part[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = (lane >> 4) * 8 + h * 4 + ((lane >> 2) & 3);
+        const int row = r0 + (lane >> 4) * 8 + h * 4 + ((lane >> 2) & 3);
         const int col = i0 + (lane & 3) * 4;
         const char* p = lds + (row * chunks + place(row, col >> 3)) * 16 +
                         (col & 7) * 2;
@@ -173,22 +174,23 @@ struct Tile {
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       const int row = i0 + (lane & 15);
-      const int chunk = lane >> 4;
+      const int chunk = (r0 >> 3) + (lane >> 4);
       return *(const s16x8*)(lds + (row * chunks + place(row, chunk)) * 16);
     }
   }
 };
 
-// A tile's fragments of a wave.
-template <int BI, int BJ, int FI, int FJ, bool PT, bool QT>
+// A wave's fragments of 32 r of a tile of KR.
+template <int BI, int BJ, int FI, int FJ, bool PT, bool QT, int KR>
 struct Fragments {
   s16x8 p[FI], q[FJ];
-  __device__ __forceinline__ void read(const char* lds, int wi, int wj) {
+  __device__ __forceinline__ void read(const char* lds, int wi, int wj, int r0 = 0) {
+    using P = Tile<BI, PT, KR>;
 #pragma unroll
-    for (int x = 0; x < FI; ++x) p[x] = Tile<BI, PT>::fragment(lds, wi + x * 16);
+    for (int x = 0; x < FI; ++x) p[x] = P::fragment(lds, wi + x * 16, r0);
 #pragma unroll
     for (int y = 0; y < FJ; ++y)
-      q[y] = Tile<BJ, QT>::fragment(lds + Tile<BI, PT>::bytes, wj + y * 16);
+      q[y] = Tile<BJ, QT, KR>::fragment(lds + P::bytes, wj + y * 16, r0);
   }
 };
 
@@ -196,11 +198,10 @@ struct Fragments {
 // matrix instructions. (With the reads spread evenly over all of them, or left to
 // the compiler, the products of 16384 x 4096 x 2048 run at 966 to 1200 TFLOP/s,
 // so at 1142 to 1213.)
-template <int READS, int WRITES = 0>
+template <int READS>
 __device__ __forceinline__ void spread() {
 #pragma unroll
   for (int i = 0; i < READS; ++i) {
-    if (i < WRITES) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);   // a write
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                   // a read
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                   // a product
   }
@@ -212,7 +213,7 @@ __device__ __forceinline__ void spread() {
 // condition, and waits can count them.
 template <typename T, int B, bool TR, int NT>
 struct Staged {
-  using L = Tile<B, TR>;
+  using L = Tile<B, TR, kSR>;
   static constexpr int n = L::rows * L::chunks / NT;
   const T* tile;              // the same for all lanes; moves on with each tile
   int32_t offset[n];          // bytes from there; stays
@@ -251,7 +252,7 @@ struct Staged {
     int32_t o[n];
 #pragma unroll
     for (int k = 0; k < n; ++k) o[k] = offset[k];
-    if (TR ? left < kR : columns < kR) {
+    if (TR ? left < kSR : columns < kSR) {
 #pragma unroll
       for (int k = 0; k < n; ++k) {
         if constexpr (TR) {
@@ -267,8 +268,8 @@ struct Staged {
     for (int k = 0; k < n; ++k) __builtin_memcpy(&v[k], (const char*)tile + o[k], 16);
   }
   __device__ __forceinline__ void next(int64_t stride) {
-    tile += TR ? kR * stride : kR;
-    columns -= kR;
+    tile += TR ? kSR * stride : kSR;
+    columns -= kSR;
   }
 
   // columns_, left: of the tile that v holds
@@ -278,7 +279,7 @@ struct Staged {
     for (int k = 0; k < n; ++k) {
       const int row = row_of(k), chunk = chunk_of(k);
       s16x8 x = v[k];
-      if (TR ? edge || left < kR : columns_ < kR) {
+      if (TR ? edge || left < kSR : columns_ < kSR) {
         int by = TR ? back[k] : chunk * 8 - ((int)columns_ - 8);
         by = by < 0 ? 0 : by > 8 || (TR && row >= left) ? 8 : by;
         x = moved(x, by);
@@ -396,26 +397,27 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
 }
 
 // BI x BJ of the output by WI x WJ waves, operands at any alignment. While a tile
-// is multiplied, the next one's fragments are read, the one after goes from
-// registers to LDS, and the four after that are under way into four sets of
-// registers.
+// is multiplied, the next one goes from registers to LDS, and the two after that are
+// under way into two sets of registers. (Tiles of 32 r, four under way, take 43 us
+// for 32768 x 997 by 256 where these take 39.7: a row's 128-byte line is then asked
+// for twice, and the second request waits for the first.)
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ __launch_bounds__(WI * WJ * 64, 2)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
-  constexpr int kPBytes = Tile<BI, PT>::bytes;
-  constexpr int kBytes = kPBytes + Tile<BJ, QT>::bytes;
+  constexpr int kPBytes = Tile<BI, PT, kSR>::bytes;
+  constexpr int kBytes = kPBytes + Tile<BJ, QT, kSR>::bytes;
   using P = Staged<T, BI, PT, NT>;
   using Q = Staged<T, BJ, QT, NT>;
-  __shared__ __attribute__((aligned(16))) char lds[kStages * kBytes];
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
   const int wave = threadIdx.x >> 6;
   const Place at = map.place(blockIdx.x);
   const int64_t i0 = (int64_t)at.i * BI, j0 = (int64_t)at.j * BJ;
   const int wi = wave / WJ * (BI / WI), wj = wave % WJ * (BJ / WJ);
   // this block's part of r, whole tiles
-  const int tiles = (int)((a.r + kR - 1) / kR);
+  const int tiles = (int)((a.r + kSR - 1) / kSR);
   const int first = (int)((int64_t)tiles * at.split / a.splits);
   const int count = (int)((int64_t)tiles * (at.split + 1) / a.splits) - first;
   f32x4 acc[FI][FJ];
@@ -425,16 +427,16 @@ void product_kernel(Product a, Tiles map) {
     for (int y = 0; y < FJ; ++y) acc[x][y] = (f32x4)0.f;
   P p;
   Q q;
-  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kR, a.p_cols);
-  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kR, a.q_cols);
+  p.start((const T*)a.p, a.p_stride, i0, a.i, (int64_t)first * kSR, a.p_cols);
+  q.start((const T*)a.q, a.q_stride, j0, a.j, (int64_t)first * kSR, a.q_cols);
   const bool edge_p = a.p_cols - i0 < BI, edge_q = a.q_cols - j0 < BJ;
-  s16x8 vp[kStages][P::n], vq[kStages][Q::n];
+  s16x8 vp[2][P::n], vq[2][Q::n];
   // a tile's r from its first on, and its rows' columns, as they are stored
-  const int64_t left0 = a.r - (int64_t)first * kR;
+  const int64_t left0 = a.r - (int64_t)first * kSR;
   const int64_t p_columns = p.columns, q_columns = q.columns;
   int loaded = 0;
   auto load = [&](int set) {          // the next tile, the last one for ever
-    const int64_t left = left0 - (int64_t)loaded * kR;
+    const int64_t left = left0 - (int64_t)loaded * kSR;
     p.load(vp[set], a.p_stride, left);
     q.load(vq[set], a.q_stride, left);
     if (loaded + 1 < count) {
@@ -444,42 +446,38 @@ void product_kernel(Product a, Tiles map) {
     }
   };
   auto store = [&](int set, int t) {
-    const int64_t done = (int64_t)t * kR;
+    const int64_t done = (int64_t)t * kSR;
     p.store(vp[set], lds + set * kBytes, left0 - done, p_columns - done, edge_p);
     q.store(vq[set], lds + set * kBytes + kPBytes, left0 - done, q_columns - done, edge_q);
   };
-  using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
+  using F = Fragments<BI, BJ, FI, FJ, PT, QT, kSR>;
   F one, two;
-#pragma unroll
-  for (int k = 0; k < kStages; ++k) load(k);
-  store(0, 0);
-  load(0);
-  store(1, 1);
-  load(1);
-  __syncthreads();
-  one.read(lds, wi, wj);
-  // the tile t % 4 == k
-  auto step = [&](int t, int k, const F& now, F& next) {
-    __syncthreads();
-    store((k + 2) & 3, t + 2);
-    load((k + 2) & 3);
-    next.read(lds + ((k + 1) & 3) * kBytes, wi, wj);
+  auto multiply = [&](const F& f) {
 #pragma unroll
     for (int x = 0; x < FI; ++x)
 #pragma unroll
-      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(now.q[y], now.p[x], acc[x][y], T());
-    spread<kReads, P::n + Q::n>();
+      for (int y = 0; y < FJ; ++y) acc[x][y] = mma(f.q[y], f.p[x], acc[x][y], T());
+  };
+  load(0);
+  load(1);
+  store(0, 0);
+  load(0);
+  // tile t lies in LDS t % 2, tile t + 1 in registers (t + 1) % 2
+  auto step = [&](int t, int k) {
+    __syncthreads();
+    one.read(lds + k * kBytes, wi, wj, 0);
+    two.read(lds + k * kBytes, wi, wj, 32);
+    multiply(one);
+    store(k ^ 1, t + 1);
+    load(k ^ 1);
+    multiply(two);
   };
   int t = 0;
-  for (; t + 4 <= count; t += 4) {
-    step(t, 0, one, two);
-    step(t + 1, 1, two, one);
-    step(t + 2, 2, one, two);
-    step(t + 3, 3, two, one);
+  for (; t + 2 <= count; t += 2) {
+    step(t, 0);
+    step(t + 1, 1);
   }
-  if (t < count) step(t, 0, one, two);
-  if (t + 1 < count) step(t + 1, 1, two, one);
-  if (t + 2 < count) step(t + 2, 2, one, two);
+  if (t < count) step(t, 0);
   __syncthreads();
   static_assert(WI * WJ * put_bytes<FJ, 2>() <= sizeof(lds), "LDS");
   put<T, FI, FJ, 2, EPI>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi,
@@ -509,7 +507,7 @@ __device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
 // there. Chunks behind r's end come from a block of zeros.
 template <typename T, int B, bool TR, int NT>
 struct Direct {
-  using L = Tile<B, TR>;
+  using L = Tile<B, TR, kR>;
   static constexpr int n = L::rows * L::chunks / NT;
   const T* tile;              // the same for all lanes; moves on with each tile
   uint32_t offset[n];         // bytes from there; stays
@@ -570,8 +568,8 @@ void product_direct_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
-  constexpr int kPBytes = Tile<BI, PT>::bytes;
-  constexpr int kBytes = kPBytes + Tile<BJ, QT>::bytes;
+  constexpr int kPBytes = Tile<BI, PT, kR>::bytes;
+  constexpr int kBytes = kPBytes + Tile<BJ, QT, kR>::bytes;
   constexpr int kLoads = Direct<T, BI, PT, NT>::n + Direct<T, BJ, QT, NT>::n;
   // s_waitcnt: at most S - 2 tiles' loads under way, no LDS read
   constexpr int kLeave = (S - 2) * kLoads, kFirst = (S - 1) * kLoads;
@@ -603,7 +601,7 @@ void product_direct_kernel(Product a, Tiles map) {
     q.load(lds0 + stage + kPBytes, a.q_stride);
     stage = stage == (S - 1) * kBytes ? 0 : stage + kBytes;
   };
-  using F = Fragments<BI, BJ, FI, FJ, PT, QT>;
+  using F = Fragments<BI, BJ, FI, FJ, PT, QT, kR>;
   int ready = kBytes;                                    // the tile to read next
   auto step = [&](const F& now, F& next) {
     __builtin_amdgcn_s_waitcnt(kWait);
