@@ -680,23 +680,23 @@ void sort_spans(std::vector<Span>& v) {
 
 // -> norm; scales into `outs`, or in place without them
 Tensor clip_grad_norm(std::vector<Tensor> grads,
-                                   c10::optional<std::vector<Tensor>> outs,
-                                   int64_t order, double max_norm, double eps,
-                                   bool scale) {
+                      c10::optional<std::vector<Tensor>> outs, int64_t order,
+                      double max_norm, double eps, bool scale) {
   TORCH_CHECK_VALUE(!grads.empty(), "no tensors were given");
   TORCH_CHECK_VALUE(!outs.has_value() || outs->size() == grads.size(),
                     "out must have as many tensors as the list");
   const Tensor first = grads[0];
   TORCH_CHECK_VALUE(first.is_cuda(), "the tensors must be on a GPU");
   const c10::DeviceGuard guard(first.device());
-  const int count = (int)grads.size();
-  std::vector<blk::GradTensor> g(count);
+  static constexpr int kSize[3] = {4, 2, 2};
+  const int listed = (int)grads.size();
+  std::vector<blk::GradTensor> g(listed);
   std::vector<Tensor> kept;                         // copies that the kernels use
   std::vector<std::pair<Tensor, Tensor>> back;      // (where it belongs, copy)
   std::vector<Span> read, written;
-  if (scale) written.reserve(count);
-  if (scale && outs.has_value()) read.reserve(count);
-  for (int i = 0; i < count; ++i) {
+  if (scale) written.reserve(listed);
+  if (scale && outs.has_value()) read.reserve(listed);
+  for (int i = 0; i < listed; ++i) {
     Tensor in = grads[i];
     TORCH_CHECK_TYPE(in.layout() == torch::kStrided, "sparse tensors are not taken");
     check_device(in, first, "a tensor");
@@ -748,6 +748,26 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
                         "an output shares memory with a tensor of the list");
       if (read[i].hi <= written[j].lo) ++i; else ++j;
     }
+  }
+  for (size_t i = 0; i < back.size(); ++i)
+    for (size_t j = 0; j < i; ++j)
+      TORCH_CHECK_VALUE(back[i].first.data_ptr() != back[j].first.data_ptr(),
+                        "two of the tensors to be written share memory");
+  // neighbours in memory are one tensor to the kernels: a bucket's views end to end
+  // are one entry instead of a thousand
+  int count = 0;
+  for (int i = 0; i < listed; ++i) {
+    if (!g[i].numel) continue;
+    if (count) {
+      blk::GradTensor& last = g[count - 1];
+      if (last.in_dtype == g[i].in_dtype && last.out_dtype == g[i].out_dtype &&
+          (const char*)last.in + last.numel * kSize[last.in_dtype] == g[i].in &&
+          (char*)last.out + last.numel * kSize[last.out_dtype] == g[i].out) {
+        last.numel += g[i].numel;
+        continue;
+      }
+    }
+    g[count++] = g[i];
   }
   int64_t chunk = 0;
   const int64_t blocks = blk::grad_norm_blocks(g.data(), count, &chunk);

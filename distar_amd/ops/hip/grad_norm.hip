@@ -6,8 +6,8 @@
 // Memory bounds both: the norm reads every value once, the scaling reads and
 // writes each once more, and not at all in place when nothing is clipped. The
 // tensors' addresses and sizes travel in the kernel's arguments (4 KB hold some
-// 230 tensors, or 160 with outputs), so no table is copied to the device and a
-// captured graph keeps its own. A block takes one chunk of one tensor and leaves
+// 230 tensors, or 160 with outputs; neighbours in memory count as one), so no table
+// is copied to the device and a captured graph keeps its own. A block takes one chunk of one tensor and leaves
 // one partial sum; a last block adds those up in a fixed order. Sums over more
 // than 8 elements are 64-bit, so they neither overflow nor drift.
 //

@@ -432,6 +432,28 @@ def test_clip_grad_norm_many_strided_and_neighbours(device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+def test_clip_grad_norm_bucket_views(device):
+    gen = torch.Generator().manual_seed(3)
+    sizes = [1, 7, 300, 0, 8192, 5, 16385, 40000]
+    bucket = torch.randn(sum(sizes), generator=gen).to(device, torch.bfloat16)
+    out = torch.full((sum(sizes),), math.nan, device=device)
+    want = torch.linalg.vector_norm(bucket.double())
+    scale = 0.5 / (float(want) + 1e-6)
+    for order in (list(range(8)), [3, 1, 0, 2, 7, 6, 5, 4]):   # in memory's order, and not
+        grads, outs = ([list(t.split(sizes))[i] for i in order] for t in (bucket, out))
+        near(clip_grad_norm(grads, 0.5, out=outs), want, 2 * U * want)
+        near(out, bucket.double() * scale, 8 * U * bucket.double().abs() * scale)
+    # neighbours on one side only, and another type between neighbours
+    apart = [torch.empty(n, device=device) for n in sizes]
+    clip_grad_norm(list(bucket.split(sizes)), 0.5, out=apart)
+    assert torch.equal(torch.cat(apart), out)
+    mixed = list(bucket.split(sizes))
+    mixed[2] = mixed[2].float()
+    clip_grad_norm(mixed, 0.5, out=apart)
+    near(torch.cat(apart), bucket.double() * scale, 8 * U * bucket.double().abs() * scale)
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_clip_grad_norm_extremes(device):
     big = [torch.full((1000,), 1e30, device=device), torch.full((3,), -1e37, device=device)]
     want = torch.linalg.vector_norm(torch.cat(big).double())
@@ -471,7 +493,8 @@ def test_clip_grad_norm_refusals(device):
             grad_norm([g.double()])
         with pytest.raises(ValueError):
             grad_norm([g, g.cpu()])
-        for bad in ([g, g], [g[:6], g[5:]], [g[5:], g[:6]]):
+        wide = torch.ones(6, 4, device=device)
+        for bad in ([g, g], [g[:6], g[5:]], [g[5:], g[:6]], [wide[:, :2], wide[:, :2]]):
             with pytest.raises(ValueError):
                 clip_grad_norm(bad, 1.)
         with pytest.raises(ValueError):
