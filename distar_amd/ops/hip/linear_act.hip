@@ -494,11 +494,11 @@ __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 // loads write no register, and the kernel counts and waits for them itself.
 __device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :: "v"(offset), "s"(base), "s"(lds) : "memory");
+               :: "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :: "v"(from), "s"(lds) : "memory");
+               :: "v"(from), "s"(lds) : "memory", "m0");
 }
 
 // A tile's loads where every chunk of 8 is wholly inside or outside the operand

@@ -586,7 +586,8 @@ def test_linear_act(device, dtype, rows, k, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', LOW)
-@pytest.mark.parametrize('rows,k,n', [(2600, 72, 2568), (520, 2568, 2568), (2600, 2568, 40), (5000, 256, 1024)])
+@pytest.mark.parametrize('rows,k,n', [(2600, 72, 2568), (520, 2568, 2568), (2600, 2568, 40), (5000, 256, 1024),
+                                      (3600, 1032, 3400), (3600, 3400, 1032), (4104, 2600, 2600)])
 def test_linear_act_large(dtype, rows, k, n):
     gen = torch.Generator('cuda').manual_seed(rows + k + n)
     make = lambda *s: torch.randn(*s, generator=gen, device='cuda').to(dtype)  # noqa: E731
@@ -854,3 +855,68 @@ def test_inference_alternatives_and_fused_norm_blocks(device):
     x = torch.randn(5, 24, device=device)
     torch.testing.assert_close(fused(x), plain(x), rtol=1e-5, atol=1e-5)
     assert build_normalization('FusedLN', dim=1) is FusedLayerNorm
+
+
+# ------------------------------------------------------------------ sizes and streams
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    gen = torch.Generator('cuda').manual_seed(0)
+    x = torch.randn(70001, 32000, generator=gen, device='cuda', dtype=torch.bfloat16)     # 2.2e9 elements
+    w, b = torch.randn(2, 32000, generator=gen, device='cuda')
+    y = layer_norm(x, w, b)
+    for part in (slice(0, 2), slice(67105, 67112), slice(-3, None)):
+        assert torch.equal(y[part], layer_norm(x[part], w, b))
+    del y
+    tokens = torch.randint(0, 32000, (70001,), generator=gen, device='cuda')
+    leaf = x.requires_grad_()
+    got = token_logprobs(leaf, tokens, top_k=2)
+    d, = torch.autograd.grad(got.logprob.sum(), leaf)
+    for part in (slice(0, 2), slice(67105, 67112), slice(-3, None)):
+        some = x.detach()[part].clone().requires_grad_()
+        ref = token_logprobs(some, tokens[part], top_k=2)
+        assert torch.equal(got.top_tokens[part], ref.top_tokens)
+        torch.testing.assert_close(got.logprob[part], ref.logprob, rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(d[part], torch.autograd.grad(ref.logprob.sum(), some)[0], rtol=1e-2, atol=1e-5)
+    del d, got
+    x = x.detach()
+    weight = torch.randn(24, 32000, generator=gen, device='cuda').bfloat16() * 0.01
+    y = linear_act(x, weight, None, 'relu')
+    torch.testing.assert_close(y[-200:], linear_act(x[-200:].clone(), weight, None, 'relu'))
+    wide = linear_act(y, weight.t().contiguous()[:, :24])                                # 2.2e9 outputs
+    torch.testing.assert_close(wide[-200:], linear_act(y[-200:], weight.t().contiguous()))
+    del wide, y
+    x.fill_(1.0)
+    want = math.sqrt(70001 * 32000)
+    norm = clip_grad_norm([x], want / 2)
+    assert abs(float(norm) - want) <= 4 * U * want
+    assert bool((x[-1] == 0.5).all()) and bool((x[0] == 0.5).all()) and bool((x[67108] == 0.5).all())
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    def work(seed):
+        gen = torch.Generator('cuda').manual_seed(seed)
+        x = torch.randn(3000, 264, generator=gen, device='cuda').bfloat16().requires_grad_()
+        w = torch.randn(520, 264, generator=gen, device='cuda').bfloat16().requires_grad_()
+        t = torch.randint(0, 520, (3000,), generator=gen, device='cuda')
+        return x, w, t
+
+    def run(x, w, t):
+        y = linear_act(layer_norm(x), w, None, 'silu')
+        got = token_logprobs(y, t, top_k=4)
+        grads = torch.autograd.grad(got.logprob.sum() + got.entropy.sum(), [x, w])
+        return [got.logprob.detach(), got.top_tokens, clip_grad_norm(grads, 1.0), *grads]
+
+    inputs = [work(1), work(2)]
+    want = [run(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for _ in range(3):
+        got = []
+        for stream, i in zip(streams, inputs):
+            with torch.cuda.stream(stream):
+                got.append(run(*i))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
