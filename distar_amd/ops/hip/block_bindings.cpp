@@ -323,9 +323,12 @@ std::array<Tensor, 5> token_logprobs_fwd(Tensor logits, Tensor tokens, OptTensor
   const int64_t rows = r.logits.rows;
   const int64_t k = std::min<int64_t>(top_k, logits.size(-1));
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= 64, "top_k must be 0 to 64, got ", top_k);
-  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite((float)(1.0 / temperature)) &&
-                        std::isfinite(temperature),
-                    "temperature must be positive, got ", temperature);
+  // beyond that the scaled logits or their scale leave the 32-bit range
+  TORCH_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e30,
+                    "temperature must be positive, 1e-30 to 1e30, got ", temperature);
+  // a launch has at most 2^32 threads, and a thread of the gradient takes 32 bytes
+  TORCH_CHECK_VALUE(!stats || logits.numel() < (int64_t)1 << 34, "logits of ",
+                    logits.numel(), " elements are too large for a gradient");
   const auto f32 = logits.options().dtype(torch::kFloat32);
   Tensor logprob = torch::empty(tokens.sizes(), f32);
   Tensor entropy = torch::empty(tokens.sizes(), f32);
@@ -465,7 +468,8 @@ Rows weight_rows_of(const Tensor& in) {
 void run_product(blk::Product& a, int dtype, const Tensor& like) {
   TORCH_CHECK_VALUE(a.i < (int64_t)1 << 32 && a.r < (int64_t)1 << 32,
                     "more than 2^32 rows");
-  TORCH_CHECK_VALUE(((a.i + 127) / 128) * ((a.j + 127) / 128) < (int64_t)1 << 30,
+  // a launch has at most 2^32 threads
+  TORCH_CHECK_VALUE(((a.i + 127) / 128) * ((a.j + 127) / 128) < (int64_t)1 << 24,
                     "a product of ", a.i, " by ", a.j, " is too large");
   a.splits = blk::product_splits(a);
   Tensor partial;

@@ -323,20 +323,23 @@ template <typename WT>
 __global__ __launch_bounds__(1024) void ln_join_kernel(LayerNormBwd a) {
   __shared__ float lds[64][17];
   const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
-  const int64_t c = (int64_t)blockIdx.x * 16 + lane;
   const int64_t cols = 2 * (int64_t)a.width;
-  float v = 0.f;
-  if (c < cols)
+  for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < cols; c0 += (int64_t)gridDim.x * 16) {
+    const int64_t c = c0 + lane;
+    float v = 0.f;
+    if (c < cols)
 #pragma unroll 4
-    for (int k = group; k < a.blocks; k += 64) v += a.partial[k * cols + c];
-  lds[group][lane] = v;
-  __syncthreads();
-  if (group == 0 && c < cols) {
-    for (int k = 1; k < 64; ++k) v += lds[k][lane];
-    if (c < a.width)
-      ((WT*)a.dweight)[c] = (WT)v;
-    else
-      ((WT*)a.dbias)[c - a.width] = (WT)v;
+      for (int k = group; k < a.blocks; k += 64) v += a.partial[k * cols + c];
+    lds[group][lane] = v;
+    __syncthreads();
+    if (group == 0 && c < cols) {
+      for (int k = 1; k < 64; ++k) v += lds[k][lane];
+      if (c < a.width)
+        ((WT*)a.dweight)[c] = (WT)v;
+      else
+        ((WT*)a.dbias)[c - a.width] = (WT)v;
+    }
+    __syncthreads();
   }
 }
 
@@ -407,9 +410,11 @@ void bwd(const LayerNormBwd& a, hipStream_t stream) {
       ln_columns_kernel<T><<<dim3((a.width + 255) / 256, a.blocks), 256, 0,
                              stream>>>(a);
   }
-  if (a.partial)
-    ln_join_kernel<WT><<<dim3((2 * (int64_t)a.width + 15) / 16), 1024, 0,
-                         stream>>>(a);
+  if (a.partial) {
+    const int64_t need = (2 * (int64_t)a.width + 15) / 16;
+    const dim3 columns((unsigned)(need < (1 << 20) ? need : (1 << 20)));   // 2^30 threads
+    ln_join_kernel<WT><<<columns, 1024, 0, stream>>>(a);
+  }
 }
 
 }  // namespace

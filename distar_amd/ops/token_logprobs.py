@@ -97,8 +97,8 @@ def token_logprobs(logits, tokens, mask=None, temperature=1.0, top_k=0,
         raise TypeError(f'mask must be bool, not {mask.dtype}')
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f'top_k must be 0 to {MAX_TOP_K}, got {top_k}')
-    if not (1e-38 < temperature and math.isfinite(temperature)):
-        raise ValueError(f'temperature must be positive, got {temperature}')
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f'temperature must be positive, 1e-30 to 1e30, got {temperature}')
     tokens = tokens.long()
     if mask is not None:
         try:

@@ -920,3 +920,40 @@ def test_calls_on_two_streams_at_once():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_layer_norm_of_very_wide_rows():
+    # more columns than a launch has threads at 16 columns a block
+    gen = torch.Generator('cuda').manual_seed(1)
+    x, dy = torch.randn(2, 2, 2 ** 25 + 9, generator=gen, device='cuda')
+    w, b = torch.randn(2, 2 ** 25 + 9, generator=gen, device='cuda')
+    _ln_check(x, None, w, b, dy, None)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width', [9, 40, 3000])
+def test_token_logprobs_extreme_temperatures(device, dtype, width):
+    gen = torch.Generator().manual_seed(width)
+    logits = torch.randn(5, width, generator=gen).to(device, dtype)
+    logits[:, 3] = 9.
+    mask = torch.ones(5, width, dtype=torch.bool, device=device)
+    mask[:, 5] = False
+    logits[1, 6] = -math.inf
+    tokens = torch.full((5,), 3, device=device)
+    leaf = logits.clone().requires_grad_()
+    cold = token_logprobs(leaf, tokens, mask=mask, temperature=1e-30, top_k=2)
+    assert bool((cold.logprob == 0).all()) and bool((cold.entropy == 0).all())
+    assert bool((cold.top_tokens[:, 0] == 3).all()) and bool((cold.top_logprobs[:, 0] == 0).all())
+    grad, = torch.autograd.grad(cold.logprob.sum() + cold.entropy.sum(), leaf)
+    assert bool((grad == 0).all())
+    hot = token_logprobs(leaf, tokens, mask=mask, temperature=1e30)
+    # the log of the count, by a sum, a logarithm and two products
+    want = torch.full((5,), math.log(width - 1), dtype=torch.float64, device=device)
+    want[1] = math.log(width - 2)
+    near(hot.logprob, -want, (8 + width / 64) * U * (1 + want))
+    near(hot.entropy, want, (8 + width / 64) * U * (1 + want))
+    for bad in (9e-31, 2e30, math.inf, -1.):
+        with pytest.raises(ValueError):
+            token_logprobs(logits, tokens, temperature=bad)
