@@ -161,7 +161,9 @@ struct Tile {
   // together, in fours of which two ask for one chunk and two for its neighbour;
   // a turning read takes 32 bytes, so there pairs of chunks move together.
   static __device__ __forceinline__ int place(int row, int chunk) {
-    if constexpr (TR) return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
+    if constexpr (TR && B == 64)        // two rows fill the banks
+      return chunk ^ ((((row >> 1) & 1) | ((row >> 2) & 2)) << 1);
+    else if constexpr (TR) return chunk ^ (((row & 3) | ((row >> 1) & 4)) << 1);
     else if constexpr (KR == 32) return chunk ^ (-(row >> 2) & 3);
     else return chunk ^ ((row >> 1) & 7);
   }
@@ -412,7 +414,7 @@ __device__ __forceinline__ void put(const Product& a, const f32x4 (&acc)[FI][FJ]
 // for 32768 x 997 by 256 where these take 39.7: a row's 128-byte line is then asked
 // for twice, and the second request waits for the first.)
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
-__global__ __launch_bounds__(WI * WJ * 64, 2)
+__global__ __launch_bounds__(WI * WJ * 64, BI * BJ < 128 * 128 ? 4 : 2)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
@@ -570,11 +572,12 @@ struct Direct {
 // this one is in registers, so that its LDS can take the tile S further on. Every
 // step loads a tile, zeros behind r's end, so that a fixed number of loads is under
 // way and a wait can leave the youngest S - 2 tiles' alone. 256 x 256 takes four
-// tiles and a compute unit, 128 x 128 three, so that three blocks share one.
+// tiles and a compute unit, 128 x 128 three and 64 x 64 six, so that three blocks
+// share one.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ __launch_bounds__(WI * WJ * 64, BI * BJ > 128 * 128 ? 1 : 3)
 void product_direct_kernel(Product a, Tiles map) {
-  constexpr int S = BI * BJ > 128 * 128 ? 4 : 3;
+  constexpr int S = BI * BJ > 128 * 128 ? 4 : BI * BJ < 128 * 128 ? 6 : 3;
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
   constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
@@ -643,13 +646,17 @@ void product_direct_kernel(Product a, Tiles map) {
   put<T, FI, FJ, 2, EPI>(a, acc, lds + wave * put_bytes<FJ, 2>(), at.split, i0 + wi, j0 + wj);
 }
 
-// the parts of r added up in their order, and the epilogue
-template <typename T, int EPI>
+// The parts of r added up, and the epilogue. G threads take every G-th part of 8
+// values of the output, and their sums are added up in a fixed order.
+template <typename T, int EPI, int G>
 __global__ __launch_bounds__(256) void product_join_kernel(Product a) {
+  constexpr int R = 256 / G;
+  __shared__ float lds[G > 1 ? 256 : 1][8];
   const int64_t runs = (a.j + 7) / 8;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= a.i * runs) return;
-  const int64_t i = at / runs, j = at % runs * 8;
+  const int64_t at = (int64_t)blockIdx.x * R + threadIdx.x % R;
+  const int group = threadIdx.x / R;
+  const bool some = at < a.i * runs;
+  const int64_t i = some ? at / runs : 0, j = some ? at % runs * 8 : 0;
   const int n = a.j - j < 8 ? (int)(a.j - j) : 8;
   float bias[8], v[8] = {};
   s16x8 residual = (s16x8)0;
@@ -660,25 +667,32 @@ __global__ __launch_bounds__(256) void product_join_kernel(Product a) {
   const float* p = a.partial + i * a.partial_cols + j;
   const int64_t part = a.i * a.partial_cols;
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = group; s < a.splits; s += G) {
     float q[8];
     load_run<float, 8>(p + s * part, q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += q[e];
   }
-  finish<T, EPI>(a, i, j, n, v, bias, residual);
+  if constexpr (G > 1) {
+    store_run<float, 8>(lds[threadIdx.x], v);
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < G; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += lds[g * R + threadIdx.x][e];
+  }
+  if (some) finish<T, EPI>(a, i, j, n, v, bias, residual);
 }
 
 // ---- few rows
 
-constexpr int kFewRows = 64;
 constexpr int kFewWaves = 8;
 
 // 16 columns of the output for at most MT x 16 rows: what bounds a layer with few
 // rows is how soon its weights arrive, so each of 8 waves asks for an eighth of r
 // of both operands straight into fragments, and the waves' sums meet in LDS. One
-// launch, and no parts to join: 16 x 1024 by 256 takes 4.8 us, by tiles of 128
-// with r in parts 8.9 us.
+// launch, and no parts to join: 16 x 1024 by 256 takes 4.6 us, by tiles of 64
+// with r in 4 parts 9.4 us.
 template <typename T, int MT, int EPI>
 __global__ __launch_bounds__(kFewWaves * 64)
 void product_few_kernel(Product a) {
@@ -830,7 +844,14 @@ bool direct(const Product& a) {
   return chunked(a.p, a.p_stride, a.p_cols) && chunked(a.q, a.q_stride, a.q_cols);
 }
 
-bool few(const Product& a) { return a.i <= kFewRows && !a.p_t && !a.q_t; }
+// A wave's next loads wait for its last ones, so long rows go by tiles, with r in
+// parts: 64 x 1024 by 256 takes 7.2 us here, 9.6 by tiles; 64 x 4096 by 4096 21 and
+// 16; 16 x 4096 by 4096 11 and 15; 16 x 8192 by 1024 17 and 11. Unaligned rows cost
+// more here: 16 x 997 by 301 6.8 and 9.5, 16 x 2001 by 301 12.4 and 10.6.
+bool few(const Product& a) {
+  if (a.p_t || a.q_t || a.i > 64) return false;
+  return a.r <= (!direct(a) ? 1024 : a.i <= 32 ? 4096 : 2048);
+}
 
 // Tiles of 256 x 256, of which one fills a compute unit, need 1024 r to outweigh
 // their first loads and their output (32768 x 1000 by 256 takes 34 us by tiles of
@@ -840,6 +861,53 @@ bool few(const Product& a) { return a.i <= kFewRows && !a.p_t && !a.q_t; }
 bool large(const Product& a) {
   const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
   return direct(a) && ((a.r >= 1024 && tiles >= 192) || (a.r >= 4096 && tiles >= 96));
+}
+
+struct Plan {
+  int side, splits;
+};
+
+// The side of the tiles and the parts of r. Of tiles of 64 and of 128 with r in 1
+// to 512 parts it takes those that should end first, by what a block's steps of 32
+// r take where it is alone on its compute unit (at least `alone`) and for each
+// block that shares it (`shared`), and by the joining of parts: a launch, 8 bytes
+// of traffic for each value of a part, and a wait for each batch of parts. The
+// figures, in us, are fitted to 1000 timed products of 16 to 131072 rows, of which
+// the choice is 1% slower than the best of each. (In us, as chosen and by tiles of
+// 128 with parts for two blocks a compute unit: 512 x 1024 by 1024 10.5 and 20.6,
+// 2048 x 997 by 256 10.4 and 24.5, 16384 x 256 by 256 9.4 and 26.5.)
+Plan plan(const Product& a) {
+  if (large(a)) {
+    const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
+    return {256, tiles <= 128 ? 2 : 1};
+  }
+  struct Cost {
+    int side;
+    double once, alone, shared;
+  };
+  static constexpr Cost costs[2][2] = {{{64, 2.5, 0.23, 0.22}, {128, 3.5, 0.55, 0.32}},
+                                       {{64, 2.7, 0.16, 0.14}, {128, 2.9, 0.26, 0.23}}};
+  const bool whole = direct(a);
+  Plan best = {128, 1};
+  double least = 1e30;
+  for (const Cost& c : costs[whole]) {
+    const int64_t tiles = ceil_div(a.i, c.side) * ceil_div(a.j, c.side);
+    const int64_t deep = ceil_div(a.r, whole ? kR : kSR);
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256, 512}) {
+      if (s > 1 && (s * 64 > a.r || tiles * s > 1024)) break;
+      const double steps = (double)ceil_div(deep, s) * (whole ? 1 : 2);
+      const double share = c.shared * (double)(tiles * s) / 256;
+      double t = c.once + steps * (share > c.alone ? share : c.alone);
+      if (s > 1)
+        t += 2.3 + 8e-6 / 5.5 * (double)a.i * (double)a.j * s +
+             0.64 * (double)ceil_div(s, s >= 64 ? 128 : s >= 8 ? 32 : 4);
+      if (t < least) {
+        least = t;
+        best = {c.side, s};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, bool PT, bool QT, int EPI>
@@ -853,21 +921,30 @@ void launch(const Product& a, hipStream_t stream) {
       return;
     }
   }
-  const int side = large(a) ? 256 : 128;
+  const int side = plan(a).side;
   const Tiles map = {(int)ceil_div(a.i, side), (int)ceil_div(a.j, side), a.splits};
   const dim3 grid((unsigned)map.i * map.j * map.splits);
-  if (large(a))
+  if (side == 256)
     product_direct_kernel<T, 256, 256, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
-  else if (direct(a))
+  else if (direct(a) && side == 128)
     product_direct_kernel<T, 128, 128, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
-  else
+  else if (direct(a))
+    product_direct_kernel<T, 64, 64, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
+  else if (side == 128)
     product_kernel<T, 128, 128, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
+  else
+    product_kernel<T, 64, 64, 2, 2, PT, QT, EPI><<<grid, 256, 0, stream>>>(a, map);
 }
 
 template <typename T, int EPI>
 void join(const Product& a, hipStream_t stream) {
-  product_join_kernel<T, EPI><<<dim3((unsigned)ceil_div(a.i * ceil_div(a.j, 8), 256)),
-                                256, 0, stream>>>(a);
+  const int64_t runs = a.i * ceil_div(a.j, 8);
+  if (a.splits >= 64)
+    product_join_kernel<T, EPI, 32><<<dim3((unsigned)ceil_div(runs, 8)), 256, 0, stream>>>(a);
+  else if (a.splits >= 8)
+    product_join_kernel<T, EPI, 8><<<dim3((unsigned)ceil_div(runs, 32)), 256, 0, stream>>>(a);
+  else
+    product_join_kernel<T, EPI, 1><<<dim3((unsigned)ceil_div(runs, 256)), 256, 0, stream>>>(a);
 }
 
 template <typename T>
@@ -906,18 +983,7 @@ void launch_act_bwd(const ActBwd& a, hipStream_t stream) {
 
 }  // namespace
 
-int product_splits(const Product& a) {
-  if (few(a)) return 1;
-  if (large(a)) {
-    const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
-    return tiles <= 128 ? 2 : 1;
-  }
-  const int64_t tiles = ceil_div(a.i, 128) * ceil_div(a.j, 128);
-  const int64_t deep = ceil_div(a.r, kR);
-  int64_t s = 512 / tiles;
-  s = s < deep / 4 ? s : deep / 4;
-  return s < 1 ? 1 : (int)s;
-}
+int product_splits(const Product& a) { return few(a) ? 1 : plan(a).splits; }
 
 void product(const Product& a, int dtype, hipStream_t stream) {
   if (dtype == kBF16) launch_any<bf16>(a, stream);

@@ -957,3 +957,16 @@ def test_token_logprobs_extreme_temperatures(device, dtype, width):
     for bad in (9e-31, 2e30, math.inf, -1.):
         with pytest.raises(ValueError):
             token_logprobs(logits, tokens, temperature=bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', LOW)
+@pytest.mark.parametrize('rows,k,n', [(512, 1024, 1024), (1024, 384, 1000), (2048, 997, 256), (600, 1201, 1003), (30000, 64, 136),
+                                      (20000, 33, 41), (5000, 333, 777), (48, 3001, 200), (20, 4104, 264), (64, 2048, 520),
+                                      (40, 4096, 1000), (100, 1500, 8)])
+def test_linear_act_tiles_and_parts(dtype, rows, k, n):
+    gen = torch.Generator('cuda').manual_seed(rows + k + n)
+    make = lambda *s: torch.randn(*s, generator=gen, device='cuda').to(dtype)  # noqa: E731
+    x, w, b, dy, r = make(rows, k), (make(n, k) * k ** -0.5).to(dtype), make(n), make(rows, n), make(rows, n)
+    _linear_check(x, w, b, 'silu', r, dy)
+    _linear_check(x, w, b, 'relu', None, dy)
