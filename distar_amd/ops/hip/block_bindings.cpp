@@ -569,7 +569,7 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
     blk::ActBwd b{};
     b.blocks = blk::act_bwd_blocks(rows, n);
     Tensor partial;
-    if (need_b)
+    if (need_b && b.blocks > 1)
       partial = torch::empty({b.blocks * n}, x.options().dtype(torch::kFloat32));
     b.dy = yr.t.data_ptr();
     if (act) {
@@ -577,7 +577,7 @@ std::array<Tensor, 3> linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor 
       b.z = saved.data_ptr();
       b.dz = dz.data_ptr();
     }
-    b.partial = need_b ? partial.data_ptr<float>() : nullptr;
+    b.partial = partial.defined() ? partial.data_ptr<float>() : nullptr;
     b.dbias = need_b ? db.data_ptr() : nullptr;
     b.dbias_f32 = bias_type == torch::kFloat32;
     b.rows = rows;
