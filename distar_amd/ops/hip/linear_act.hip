@@ -860,13 +860,13 @@ bool few(const Product& a) {
 }
 
 // Tiles of 256 x 256, of which one fills a compute unit, need 1024 r to outweigh
-// their first loads and their output (32768 x 1000 by 256 takes 34 us by tiles of
-// 128, 52 us by these), and either enough of them for all compute units or enough
-// r to share a tile among two blocks (with 128 tiles of only 1024 r, 2048 x 1024 by
-// 4096 takes 49 us in two parts, 29 us by tiles of 128).
+// their first loads (bare, 16384 x 1024 by 4096 takes 164 us by tiles of 128, 151 us
+// by these; 32768 x 1000 by 256 34 and 52) and 2048 where nothing hides an activation
+// behind them (with gelu 183 and 192; 8192 x 2048 by 2048 86 and 75), and either
+// enough of them for all compute units or enough r to share a tile among two blocks.
 bool large(const Product& a) {
   const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
-  return direct(a) && ((a.r >= 1024 && tiles >= 192) || (a.r >= 4096 && tiles >= 96));
+  return direct(a) && ((a.r >= (a.act ? 2048 : 1024) && tiles >= 192) || (a.r >= 4096 && tiles >= 96));
 }
 
 struct Plan {

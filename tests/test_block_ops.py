@@ -963,7 +963,7 @@ def test_token_logprobs_extreme_temperatures(device, dtype, width):
 @pytest.mark.parametrize('dtype', LOW)
 @pytest.mark.parametrize('rows,k,n', [(512, 1024, 1024), (1024, 384, 1000), (2048, 997, 256), (600, 1201, 1003), (30000, 64, 136),
                                       (20000, 33, 41), (5000, 333, 777), (48, 3001, 200), (20, 4104, 264), (64, 2048, 520),
-                                      (40, 4096, 1000), (100, 1500, 8)])
+                                      (40, 4096, 1000), (100, 1500, 8), (4104, 3000, 4104)])
 def test_linear_act_tiles_and_parts(dtype, rows, k, n):
     gen = torch.Generator('cuda').manual_seed(rows + k + n)
     make = lambda *s: torch.randn(*s, generator=gen, device='cuda').to(dtype)  # noqa: E731
