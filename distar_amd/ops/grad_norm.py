@@ -67,7 +67,8 @@ def clip_grad_norm(tensors, max_norm, norm_type=2.0, eps=1e-6, out=None):
 
     In place, or into `out`: a list of tensors of the same shapes in types of
     their own, such as float32 gradients of an optimiser.  Tensors that are
-    written must not share memory with each other.  A norm of NaN makes the
+    written must not share memory with each other, nor with others of `tensors`
+    (one may be its own output).  A norm of NaN makes the
     results NaN, an infinite one makes them 0 (and infinities NaN), as the
     formula says.
     """

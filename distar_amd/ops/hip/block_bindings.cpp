@@ -719,7 +719,9 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
       TORCH_CHECK_VALUE(dense_out, "an output must be dense, without gaps or overlaps");
       if (g[i].numel) {
         written.push_back(span_of(out));
-        if (dense) read.push_back(span_of(in));
+        const bool itself = out.data_ptr() == in.data_ptr() && out.strides() == in.strides() &&
+                            out.scalar_type() == in.scalar_type();
+        if (dense && !itself) read.push_back(span_of(in));
       }
       if (!dense || out.strides() != in.strides()) {
         Tensor same = torch::empty_strided(out.sizes(), out.strides(), in.options());

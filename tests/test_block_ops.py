@@ -970,3 +970,17 @@ def test_linear_act_tiles_and_parts(dtype, rows, k, n):
     x, w, b, dy, r = make(rows, k), (make(n, k) * k ** -0.5).to(dtype), make(n), make(rows, n), make(rows, n)
     _linear_check(x, w, b, 'silu', r, dy)
     _linear_check(x, w, b, 'relu', None, dy)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_clip_grad_norm_own_output(device):
+    gen = torch.Generator().manual_seed(3)
+    a, b, c = (torch.randn(n, generator=gen).to(device, t) for n, t in
+               ((20003, torch.float32), (517, torch.bfloat16), (64, torch.float16)))
+    wide = torch.empty(517, device=device)
+    norm = math.sqrt(sum(float(t.double().square().sum()) for t in (a, b, c)))
+    want = [t.double() * min(1., 0.5 / (norm + 1e-6)) for t in (a, b, c)]
+    got = clip_grad_norm([a, b, c], 0.5, out=[a, wide, c])
+    near(got, torch.tensor(norm, device=device, dtype=torch.float64), 4 * U * norm)
+    for t, w in zip((a, wide, c), want):
+        near(t, w, 4 * U * w.abs())          # the norm, the quotient, the scale, a product
