@@ -984,3 +984,51 @@ def test_clip_grad_norm_own_output(device):
     near(got, torch.tensor(norm, device=device, dtype=torch.float64), 4 * U * norm)
     for t, w in zip((a, wide, c), want):
         near(t, w, 4 * U * w.abs())          # the norm, the quotient, the scale, a product
+
+
+@pytest.mark.gpu
+def test_each_operator_in_a_graph_at_several_sizes():
+    gen = torch.Generator('cuda').manual_seed(4)
+    make = lambda *s, t=torch.bfloat16: torch.randn(*s, generator=gen, device='cuda').to(t)  # noqa: E731
+
+    def norm_pass(x, r, w, b):
+        leaves = [t.detach().requires_grad_() for t in (x, r, w, b)]
+        y, s = add_layer_norm(*leaves)
+        return [y.detach(), s.detach(), *torch.autograd.grad((y * s).sum(), leaves)]
+
+    def linear_pass(x, w, b, r):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = linear_act(*leaves[:3], 'gelu', leaves[3])
+        return [y.detach(), *torch.autograd.grad(y, leaves, r)]
+
+    def logit_pass(x, tokens):
+        leaf = x.detach().requires_grad_()
+        got = token_logprobs(leaf, tokens, mask=x > -1.5, top_k=3)
+        live = got.logprob.clamp(min=-30.) + got.entropy
+        return [got.entropy.detach(), got.top_logprobs, got.top_tokens, *torch.autograd.grad(live, leaf, got.entropy)]
+
+    def clip_pass(*tensors):
+        outs = [torch.empty(t.shape, device='cuda') for t in tensors]
+        return [clip_grad_norm(list(tensors), 0.1, out=outs), *outs]
+
+    cases = [(norm_pass, [make(700, 1536), make(700, 1536), make(1536), make(1536)]),
+             (norm_pass, [make(64, 9), make(64, 9), make(9), make(9)])]
+    for m, k, n in ((40, 1024, 200), (512, 1024, 1024), (2048, 997, 256), (9000, 64, 72), (70, 5001, 33)):
+        cases.append((linear_pass, [make(m, k), make(n, k) * 0.03, make(n), make(m, n)]))
+    for m, n in ((300, 5000), (40, 327), (9, 40000)):
+        cases.append((logit_pass, [make(m, n), torch.randint(0, n, (m,), generator=gen, device='cuda')]))
+    cases.append((clip_pass, [make(3 * i * i + 1, t=TYPES[i % 3]) for i in range(300)]))
+    for run, inputs in cases:
+        run(*inputs)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(*inputs)
+        for _ in range(3):
+            inputs[0].copy_(make(*inputs[0].shape, t=inputs[0].dtype))
+            want = run(*inputs)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+        del graph, out, want
