@@ -27,7 +27,7 @@
 // (4.4 TB/s), backward 37 us (4.5 TB/s). 2048 x 24320 bf16: forward with 5
 // alternatives 30 us (3.3 TB/s), backward 33 us (6.0 TB/s; much of the logits still
 // lies in the cache behind the dies' own). 33 x 24320 fp32 with 20 alternatives:
-// 13 us, one block's latency a row; 16 x 327 fp32 with a mask and 5: 6 us.
+// 12 us, one block's latency a row; 16 x 327 fp32 with a mask and 5: 5 us.
 #include "block_common.h"
 #include "block_ops.h"
 
@@ -125,7 +125,7 @@ struct Shared {
   static constexpr int list = kList / (TPR > 64 ? 1 : 4);   // of a row or wave
   float most[waves];
   Stat stat[waves];
-  float lane_most[TPR > 64 ? waves : 1][64];
+  float lane_most[TPR > 64 ? waves : 4][64];
   float bound;
   float best_v[waves];
   int best_i[waves];
@@ -244,10 +244,8 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
   }
 }
 
-constexpr int kBatch = 4;           // runs of a thread under way together
-
-// A thread's runs of a row, TPR runs apart, a batch at a time.
-template <typename T, int TPR, bool MASKED>
+// A thread's runs of a row, TPR runs apart, kBatch of them under way together.
+template <typename T, int TPR, bool MASKED, int kBatch>
 struct Batch {
   static constexpr int V = Width<T>::v;
   Run<T> v[kBatch];
@@ -265,12 +263,14 @@ struct Batch {
     }
   }
 
-  // -inf in the places that the mask or the row's end take away
-  __device__ __forceinline__ void limit(int c0, int width) {
+  // -inf in the places that the mask or the row's end take away; first: where the
+  // first thread's runs begin
+  __device__ __forceinline__ void limit(int first, int width) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
+      if (TPR == 64 && first + j * TPR * V >= width) break;         // the same for all
       if constexpr (MASKED) v[j] = masked<T>(v[j], q[j]);
-      const RowRun<T> run(c0 + j * TPR * V, width);
+      const RowRun<T> run(first + threadIdx.x % TPR * V + j * TPR * V, width);
       if (!run.whole()) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[j][i] = run.counts(i) ? v[j][i] : (T)-kInf;
@@ -279,13 +279,16 @@ struct Batch {
   }
 };
 
-template <typename T, int TPR, bool MASKED>
-__global__ __launch_bounds__(TPR > 64 ? TPR : 256, TPR > 256 ? 2 : MASKED ? 3 : 4)
+// kBatch < 4: rows of one batch, which leave registers for more waves.
+template <typename T, int TPR, bool MASKED, int kBatch>
+__global__ __launch_bounds__(TPR > 64 ? TPR : 256,
+                             TPR > 256 ? 2 : kBatch < 4 ? (MASKED ? 5 : 6) : MASKED ? 3 : 4)
 void logprobs_kernel(LogProbs a) {
   constexpr int V = Width<T>::v;
   constexpr int RPB = TPR > 64 ? 1 : 256 / TPR;
   constexpr int W = Shared<TPR>::waves;
   constexpr int kStep = TPR * V * kBatch;
+  constexpr bool kOnce = kBatch < 4;
   __shared__ Shared<TPR> sh;
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 63;
   const int wave = TPR > 64 ? threadIdx.x >> 6 : 0;
@@ -301,7 +304,7 @@ void logprobs_kernel(LogProbs a) {
     const T* l = (const T*)a.logits + row * a.stride;
     const uint8_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
     const int64_t token = a.tokens[row];
-    Batch<T, TPR, MASKED> now;
+    Batch<T, TPR, MASKED, kBatch> now;
     if (!narrow) now.load(l, mask, t * V, width);
     // asked for behind the row's first part, whose loads it would hold up
     const float given = t == 0 ? given_logit<T>(a, row, token) : 0.f;
@@ -334,15 +337,18 @@ void logprobs_kernel(LogProbs a) {
         add(v, raise(most));
       }
     } else {
-      Batch<T, TPR, MASKED> next;
+      Batch<T, TPR, MASKED, kBatch> next;
       for (int c = 0; c < width; c += kStep) {
-        if (c + kStep < width) next.load(l, mask, c + kStep + t * V, width);
-        now.limit(c + t * V, width);
+        const bool more = !kOnce && c + kStep < width;
+        if (more) next.load(l, mask, c + kStep + t * V, width);
+        now.limit(c, width);
         float most = -kInf;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
+        for (int j = 0; j < kBatch; ++j) {
+          if (TPR == 64 && c + j * TPR * V >= width) break;         // the same for all
 #pragma unroll
           for (int i = 0; i < V; ++i) most = fmaxf(most, (float)now.v[j][i]);
+        }
         const float m = raise(most);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -350,7 +356,8 @@ void logprobs_kernel(LogProbs a) {
           forget<T>(now.v[j]);
           add(now.v[j], m);
         }
-        now = next;
+        if (kOnce) break;
+        if (TPR > 64 || more) now = next;               // a row of one batch stays
       }
     }
     const float most = st.m;              // this thread's maximum
@@ -394,16 +401,32 @@ void logprobs_kernel(LogProbs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) f((float)v[i], c + i);
     };
-    // the K-th largest of 64 lanes' maxima
+    // the K-th largest of 64 lanes' maxima: the largest K times, or the least of
+    // those with fewer than K above them (which takes as long as 6 times)
     float bound = most;
     if (TPR == 64 || wave == 0) {
       float g = most;
       if constexpr (TPR > 64)
         for (int w = 1; w < W; ++w) g = fmaxf(g, sh.lane_most[w][lane]);
-      for (int k = 0; k < K; ++k) {
-        bound = lanes_max<64>(g);
-        const uint64_t who = __ballot(g == bound);
-        if (who && lane == __ffsll((unsigned long long)who) - 1) g = -kInf;
+      if (K <= 6) {
+        for (int k = 0; k < K; ++k) {
+          bound = lanes_max<64>(g);
+          const uint64_t who = __ballot(g == bound);
+          if (who && lane == __ffsll((unsigned long long)who) - 1) g = -kInf;
+        }
+      } else {
+        sh.lane_most[slot][lane] = g;
+        row_sync<64>();
+        int above = 0;
+#pragma unroll 2
+        for (int o = 0; o < 64; o += 4) {
+          const float4 q = *(const float4*)&sh.lane_most[slot][o];
+          above += q.x > g;
+          above += q.y > g;
+          above += q.z > g;
+          above += q.w > g;
+        }
+        bound = -lanes_max<64>(above < K ? -g : -kInf);
       }
       if (lane == 0) {
         sh.count[slot] = 0;
@@ -418,10 +441,13 @@ void logprobs_kernel(LogProbs a) {
         int hit = 1;                      // a narrow row is one run
         if (!narrow) {
           hit = 0;
-          now.load(l, mask, c0, width);
-          now.limit(c0, width);
+          if (!kOnce && (TPR > 64 || width > kStep)) {
+            now.load(l, mask, c0, width);
+            now.limit(c0 - t * V, width);
+          }
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) {
+            if (TPR == 64 && c0 - t * V + j * TPR * V >= width) break;
             float r = -kInf;
 #pragma unroll
             for (int i = 0; i < V; ++i) r = fmaxf(r, (float)now.v[j][i]);
@@ -653,22 +679,24 @@ void fwd_small(const LogProbs& a, hipStream_t stream) {
   logprobs_small_kernel<T, TPR, NV, NARROW><<<grid, 256, 0, stream>>>(a);
 }
 
-template <typename T, int TPR>
+template <typename T, int TPR, int kBatch = 4>
 void fwd_as(const LogProbs& a, hipStream_t stream) {
   const int64_t rpb = TPR > 64 ? 1 : 256 / TPR;
   const int64_t need = (a.rows + rpb - 1) / rpb;
   const dim3 grid((unsigned)(need < (1 << 20) ? need : (1 << 20)));
   if (a.mask)
-    logprobs_kernel<T, TPR, true><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
+    logprobs_kernel<T, TPR, true, kBatch><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
   else
-    logprobs_kernel<T, TPR, false><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
+    logprobs_kernel<T, TPR, false, kBatch><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
 }
 
 // Rows of up to 128 runs lie in registers (65536 x 513 bf16: 17 us, 52 us by a wave
 // that runs through the row). Longer ones take a wave up to 256 runs (8192 x 2000:
-// 10 us, 47 us with 256 threads), then 256 threads (2048 x 24320: 29 us, 38 us with
+// 10 us, 47 us with 256 threads; of at most 128 runs, with alternatives, by a kernel
+// that holds no second batch: 65536 x 513 with a mask and 5 of them 84 us, 148 us by
+// the general one), then 256 threads (2048 x 24320: 29 us, 38 us with
 // 512), and 512 where rows are too few to fill the chip (33 x 24320 fp32 with 20
-// alternatives: 13.2 us, 15.5 us with 256).
+// alternatives: 12.3 us, 14.6 us with 256).
 template <typename T>
 void fwd(const LogProbs& a, hipStream_t stream) {
   const int n = (a.width + Width<T>::v - 1) / Width<T>::v;    // runs of 16 bytes
@@ -680,6 +708,10 @@ void fwd(const LogProbs& a, hipStream_t stream) {
     else if (n <= 48) fwd_small<T, 16, 3>(a, stream);
     else if (n <= 80) fwd_small<T, 16, 5>(a, stream);
     else fwd_small<T, 16, 8>(a, stream);
+  } else if (n <= 64) {
+    fwd_as<T, 64, 1>(a, stream);
+  } else if (n <= 128) {
+    fwd_as<T, 64, 2>(a, stream);
   } else if (n <= 256) {
     fwd_as<T, 64>(a, stream);
   } else if (n <= 1024 || a.rows >= 512) {

@@ -1032,3 +1032,16 @@ def test_each_operator_in_a_graph_at_several_sizes():
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
         del graph, out, want
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width,top_k', [(255, 7), (257, 7), (512, 6), (513, 64), (1024, 9), (1025, 2), (2049, 7)])
+def test_token_logprobs_alternatives_at_batch_ends(device, dtype, width, top_k):
+    gen = torch.Generator().manual_seed(width)
+    logits = (torch.randn(37, width, generator=gen) * 3).to(device, dtype)
+    tokens = torch.randint(0, width, (37,), generator=gen).to(device)
+    mask = (torch.rand(37, width, generator=gen) < 0.7).to(device)
+    mask.scatter_(-1, tokens.unsqueeze(-1), True)
+    _lp_check(logits, tokens, mask, top_k=top_k)
+    _lp_check(logits, tokens, None, temperature=0.8, top_k=top_k)
