@@ -1,4 +1,7 @@
 // Python bindings for the distar_amd HIP/CDNA4 kernels (_hip_ops).
+#include <cstdlib>
+#include <string>
+
 #include <torch/extension.h>
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -965,6 +968,11 @@ void register_block_ops(pybind11::module_& m);   // block_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_block_ops(m);
+  // read here because a look into os.environ takes longer than a launch's checks
+  m.def("disabled", [] {
+    const char* v = std::getenv("DISTAR_AMD_DISABLE_HIP");
+    return v && std::string(v) == "1";
+  }, "whether DISTAR_AMD_DISABLE_HIP is 1");
   m.def("multi_norm_sq", &multi_norm_sq,
         "K14 multi-tensor global sum-of-squares");
   m.def("multi_clip", &multi_clip,

@@ -297,7 +297,7 @@ LogitRows check_logits(const Tensor& logits, const Tensor& tokens,
   }
   TORCH_CHECK_VALUE(tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                     "tokens must have the shape of logits without its last dimension");
-  r.tokens = tokens.to(torch::kLong).contiguous();
+  r.tokens = (tokens.scalar_type() == torch::kLong ? tokens : tokens.to(torch::kLong)).contiguous();
   if (mask.has_value()) {
     check_device(*mask, logits, "mask");
     TORCH_CHECK_TYPE(mask->scalar_type() == torch::kBool, "mask must be bool");
@@ -306,7 +306,7 @@ LogitRows check_logits(const Tensor& logits, const Tensor& tokens,
       fits = mask->size(-d) == 1 || mask->size(-d) == logits.size(-d);
     TORCH_CHECK_VALUE(fits, "mask of shape ", mask->sizes(),
                       " does not broadcast to logits of shape ", logits.sizes());
-    r.mask = rows_of(mask->expand(logits.sizes()));
+    r.mask = rows_of(mask->sizes() == logits.sizes() ? *mask : mask->expand(logits.sizes()));
   }
   return r;
 }
@@ -369,7 +369,8 @@ Tensor token_logprobs_bwd(const Tensor& logits, const OptTensor& mask,
   const c10::DeviceGuard guard(logits.device());
   const Rows l = rows_of(logits);
   Rows m;
-  if (mask.has_value()) m = rows_of(mask->expand(logits.sizes()));
+  if (mask.has_value())
+    m = rows_of(mask->sizes() == logits.sizes() ? *mask : mask->expand(logits.sizes()));
   for (OptTensor* t : {&dlogprob, &dentropy})
     if (t->has_value()) *t = (*t)->to(torch::kFloat32).contiguous();
   Tensor dlogits = torch::empty(logits.sizes(), logits.options());

@@ -42,16 +42,16 @@ def maybe_ext(tensor):
     """Return the extension module for CUDA(=ROCm) tensors, None on CPU."""
     if not tensor.is_cuda:
         return None
-    if os.environ.get('DISTAR_AMD_DISABLE_HIP') == '1':
-        return None
     ext = _load()
     if ext is None:
+        if os.environ.get('DISTAR_AMD_DISABLE_HIP') == '1':
+            return None
         raise ImportError(
             'distar_amd HIP extension (_hip_ops) is not built but a GPU tensor '
             'reached a HIP-op call site. Build it in-tree with '
             '`python setup_hip.py build` (hipcc --offload-arch=gfx950); '
             'refusing to fall back to eager on GPU.')
-    return ext
+    return None if ext.disabled() else ext
 
 
 def require():

@@ -1045,3 +1045,16 @@ def test_token_logprobs_alternatives_at_batch_ends(device, dtype, width, top_k):
     mask.scatter_(-1, tokens.unsqueeze(-1), True)
     _lp_check(logits, tokens, mask, top_k=top_k)
     _lp_check(logits, tokens, None, temperature=0.8, top_k=top_k)
+
+
+@pytest.mark.gpu
+def test_kernels_are_switched_off_by_the_environment(monkeypatch):
+    from distar_amd.ops import hip_ext
+    x = torch.zeros(2, 8, device='cuda')
+    for value, off in (('1', True), ('0', False), ('', False), ('1', True), (None, False)):
+        if value is None:
+            monkeypatch.delenv('DISTAR_AMD_DISABLE_HIP')
+        else:
+            monkeypatch.setenv('DISTAR_AMD_DISABLE_HIP', value)
+        assert (hip_ext.maybe_ext(x) is None) == off
+    assert hip_ext.maybe_ext(x.cpu()) is None
