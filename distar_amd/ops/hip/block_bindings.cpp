@@ -790,7 +790,7 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
                  (float)max_norm, (float)eps, stream);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   if (scale) {
-    blk::grad_scale(g.data(), count, chunk, coef.data_ptr<float>(), stream);
+    blk::grad_scale(g.data(), count, coef.data_ptr<float>(), stream);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     for (auto& p : back) p.first.copy_(p.second);
   }

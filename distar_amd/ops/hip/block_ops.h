@@ -67,8 +67,7 @@ int64_t grad_norm_blocks(const GradTensor*, int count, int64_t* chunk);
 void grad_norm(const GradTensor*, int count, int64_t chunk, int order,
                double* partial, int64_t blocks, float* norm, float* coef,
                float max_norm, float eps, hipStream_t);
-void grad_scale(const GradTensor*, int count, int64_t chunk,
-                const float* coef, hipStream_t);
+void grad_scale(const GradTensor*, int count, const float* coef, hipStream_t);
 
 // ---- linear_act.hip
 enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
