@@ -21,7 +21,7 @@
 //
 // 262144 x 256 bf16 with a residual: forward 93 us, 5.8 TB/s over x, r, s and y;
 // backward 110 us, 4.9 TB/s over dy, ds, s and dx, and 5 us for the sums of 1024
-// blocks (a large copy reaches 4.7 TB/s). 4095 x 1536 fp32: 11, 15 and 6 us. 16 x
+// blocks (a large copy reaches 4.7 TB/s). 4095 x 1536 fp32: 11 and 20 us together. 16 x
 // 256 bf16: 2.5 us, a launch.
 #include "block_common.h"
 #include "block_ops.h"
@@ -435,7 +435,11 @@ int layer_norm_bwd_blocks(int64_t rows, int width, int dtype) {
   if (n > kMaxRuns) return rows < kWideBlocks ? (int)rows : kWideBlocks;
   const int64_t rpb = rows_a_block(n);
   const int64_t need = (rows + rpb - 1) / rpb;
-  return (int)(need < 1024 ? need : 1024);
+  // Four blocks a compute unit where a thread has one run of a row, two, with half as
+  // many partial rows, where it has two: 60000 x 1000 bf16 takes 73 us, 85 with four
+  // (111 with one), 8192 x 4096 bf16 49 and 57; one run, 20000 x 2000, 69 and 57.
+  const int64_t most = n > 256 || (n > 64 && n <= 128) ? 512 : 1024;
+  return (int)(need < most ? need : most);
 }
 
 void layer_norm_fwd(const LayerNormFwd& a, int dtype, int wdtype,
