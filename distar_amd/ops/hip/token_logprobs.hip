@@ -14,8 +14,8 @@
 //
 // The k alternatives: of 64 maxima over disjoint parts of the row (one of each
 // lane) the k-th largest is a bound that at least k elements reach, and few more
-// do. Only the few threads whose maximum reaches it read their part again; what
-// reaches it goes to a list in LDS, where each counts how many come before it, and
+// do. Only the few threads whose maximum reaches it look at their part again (read
+// again where a row is longer than the registers); what reaches it goes to a list in LDS, where each counts how many come before it, and
 // the first k write themselves out. Only a row with very many equal logits
 // overflows the list: it is searched k times instead.
 //
