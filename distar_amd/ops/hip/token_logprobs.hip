@@ -15,9 +15,10 @@
 // The k alternatives: of 64 maxima over disjoint parts of the row (one of each
 // lane) the k-th largest is a bound that at least k elements reach, and few more
 // do. Only the few threads whose maximum reaches it look at their part again (read
-// again where a row is longer than the registers); what reaches it goes to a list in LDS, where each counts how many come before it, and
-// the first k write themselves out. Only a row with very many equal logits
-// overflows the list: it is searched k times instead.
+// again where a row is longer than the registers); what reaches it goes to a list
+// in LDS, where each counts how many come before it, and the first k write
+// themselves out. Only a row with very many equal logits overflows the list: it is
+// searched k times instead.
 //
 // Backward, the gradient's memory is cut into aligned runs of 16 bytes whatever
 // the rows' width, and a run that holds the end of a row takes a slower way. The
