@@ -522,7 +522,9 @@ std::array<Tensor, 2> linear_act_fwd(Tensor x, Tensor weight, OptTensor bias,
   const Rows rr = residual.has_value() ? rows_of(*residual) : Rows{x, 0, 0};
   Tensor y = torch::empty(shape, x.options());
   Tensor z;
-  if (save) z = torch::empty(shape, x.options());
+  if (save)
+    z = torch::empty(shape, act == blk::kRelu ? x.options()
+                                              : x.options().dtype(torch::kFloat32));
   if (xr.rows) {
     blk::Product a{};
     a.p = xr.t.data_ptr();

@@ -87,14 +87,15 @@ struct Product {
   int bias_f32;
   const void *residual;                       // or null
   int64_t residual_stride;
-  void *z;                                    // what goes into act, or null
+  void *z;                                    // what goes into act, or null: float32,
+                                              // in the type for a relu
   int act;
   int splits;                                 // parts of r ...
   float *partial;                             // ... [splits][i][partial_cols],
   int64_t partial_cols;                       // j up to a multiple of 8; or null
 };
 struct ActBwd {
-  const void *dy, *z;                         // z: or null without act
+  const void *dy, *z;                         // z: Product's, or null without act
   void *dz;                                   // or null without act
   float *partial;                             // [blocks][n], or null
   void *dbias;

@@ -12,9 +12,11 @@
 // read. What lies beyond r's end is loaded as zero on both sides, what lies
 // beyond i or j is loaded from a valid place and not stored.
 //
-// z and dz are rounded to the operands' type: z is kept for the backward pass at
-// half the bytes of 32 bits, and dz is an operand of both products, which take no
-// wider type. y is computed from the 32-bit z and rounded once.
+// y is computed from the 32-bit z and rounded once. z is kept for the backward pass
+// in 32 bits too where a slope is taken from it: in the operands' type its rounding
+// would weigh as much in the gradients as that of dz, and an fp16 z could overflow
+// under a finite y. A relu needs its sign alone and keeps it in the operands' type.
+// dz is rounded to that type, because both products take no wider one.
 //
 // The matrix cores bound long r, memory the rest. 16384 x 4096 by 2048 fp16 with
 // gelu, residual and z kept: 328 us, 838 TFLOP/s (231 us, 1190 TFLOP/s, without an
@@ -95,6 +97,10 @@ __device__ __forceinline__ float act_slope(float z) {
 // What an epilogue does: an Act with bias, z and residual, or nothing.
 constexpr int kPlain = -1;
 
+// the type in which z is kept
+template <typename T, int ACT>
+using Kept = std::conditional_t<ACT == kRelu, T, float>;
+
 // The values of out[i][j ... j + 8), of which n exist: bias and residual are
 // loaded by the caller, which has many rows of them under way.
 template <typename T, int EPI>
@@ -105,7 +111,8 @@ __device__ __forceinline__ void finish(const Product& a, int64_t i, int64_t j, i
   if constexpr (EPI != kPlain) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
-    if (a.z) store_some<T, 8>((T*)a.z + at, n, v);
+    using Z = Kept<T, EPI>;
+    if (a.z) store_some<Z, 8>((Z*)a.z + at, n, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = act<EPI>(v[e]);
     if (a.residual) {
@@ -786,7 +793,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwd a) {
       for (int k = 0; k < kActRows; ++k) {
         const int64_t i = i0 + k * 8 < a.rows ? i0 + k * 8 : a.rows - 1;
         run.load((const T*)a.dy + i * a.dy_stride, d[k]);
-        if constexpr (ACT != kNone) run.load((const T*)a.z + i * a.n, z[k]);
+        if constexpr (ACT != kNone) run.load((const Kept<T, ACT>*)a.z + i * a.n, z[k]);
       }
 #pragma unroll
       for (int k = 0; k < kActRows; ++k) {

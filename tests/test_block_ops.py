@@ -1058,3 +1058,47 @@ def test_kernels_are_switched_off_by_the_environment(monkeypatch):
             monkeypatch.setenv('DISTAR_AMD_DISABLE_HIP', value)
         assert (hip_ext.maybe_ext(x) is None) == off
     assert hip_ext.maybe_ext(x.cpu()) is None
+
+
+# ------------------------------------------------------------------ corners
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', LOW)
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+@pytest.mark.parametrize('rows,n', [(5, 16), (600, 16), (700, 264)])
+def test_linear_act_slope_of_the_unrounded_sum(device, dtype, act, rows, n):
+    # an identity as the weight: z = x + b has more digits than the operands' type, and
+    # dx is dz. z comes with one 32-bit rounding, dz with the half step that `near` adds
+    # (stored twice, the second time exactly)
+    gen = torch.Generator().manual_seed(rows + n)
+    x, dy = ((torch.randn(rows, n, generator=gen) * 2).to(device, dtype) for _ in range(2))
+    b = torch.randn(n, generator=gen).to(device)
+    w, leaf = torch.eye(n, dtype=dtype, device=device), x.clone().requires_grad_()
+    dx, = torch.autograd.grad(linear_act(leaf, w, b, act, x), leaf, dy)
+    z = x.double() + b.double()
+    near(dx, dy.double() * SLOPE[act](z), dy.double().abs() * (16 * U + U * z.abs()))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+def test_linear_act_sums_beyond_fp16(device, act):
+    # z of up to 120000 either way, where the slope is 1 or 0
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(40, 16, generator=gen).to(device, torch.float16)
+    x[7] = 60000.
+    w = torch.eye(16, device=device) * 2
+    w[3:9] *= -1
+    dy = torch.randn(40, 16, generator=gen).to(device, torch.float16)
+    dy[7] /= 64                                                 # for dw is below 65504
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_(), torch.zeros(16, device=device, requires_grad=True)]
+    y = linear_act(*leaves, act)
+    assert bool((y[7, 3:9] == 0).all())
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    z = x.double() @ w.double().t()
+    dz = dy.double() * SLOPE[act](z).nan_to_num(0.)             # the formula's 0 times infinity
+    dz[7] = dy[7].double() * (z[7] > 0)
+    t = half(torch.float16)
+    off = dy.double().abs() * 32 * U + t * dz.abs() * 1.01 + torch.finfo(torch.float16).tiny
+    near(dx, dz @ w.double(), off @ w.double().abs())
+    near(dw, dz.t() @ x.double(), off.t() @ x.double().abs() + 64 * U * (dz.abs().t() @ x.double().abs()))
+    near(db, dz.sum(0), off.sum(0))
