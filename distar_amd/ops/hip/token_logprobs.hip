@@ -162,8 +162,10 @@ __device__ __forceinline__ void leave(const LogProbs& a, int64_t row, Stat st,
                  : ((given - st.m) * scale - log2sum) * kLn2;
   a.entropy[row] = h;
   if (a.stats) {
-    const float4 keep = {bad ? nan : st.m, log2sum, h,
-                         __int_as_float(ignored ? -1 : inside ? (int)token : -2)};
+    // -1: no gradient of the log probability; -2: one through the sum alone, for a
+    // token that is not possible has none of its own
+    const int place = ignored || !inside ? -1 : given == -kInf ? -2 : (int)token;
+    const float4 keep = {bad ? nan : st.m, log2sum, h, __int_as_float(place)};
     *(float4*)(a.stats + row * 4) = keep;
   }
 }

@@ -74,11 +74,11 @@ def token_logprobs(logits, tokens, mask=None, temperature=1.0, top_k=0,
     top_k: 0 to 64 alternatives, the largest logits first, equal ones by index.
 
     Returns a `TokenLogProbs`.  A row's logprob is 0 (without gradient) where its
-    token is `ignore_index`, -inf where the token is masked, NaN where it is
-    outside [0, C).  A row without any possible token has entropy 0, logprob -inf
-    and no gradient; alternatives that do not exist are token -1 with -inf.  A
-    NaN or +inf among a row's possible logits makes that row's results NaN (and
-    its alternatives -1).
+    token is `ignore_index`, -inf where the token is masked (with a gradient at the
+    possible tokens alone), NaN (without gradient) where it is outside [0, C).  A row
+    without any possible token has entropy 0, logprob -inf and no gradient;
+    alternatives that do not exist are token -1 with -inf.  A NaN or +inf among a
+    row's possible logits makes that row's results NaN (and its alternatives -1).
     """
     ext = hip_ext.maybe_ext(logits)
     if ext is not None:

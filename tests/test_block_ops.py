@@ -1102,3 +1102,39 @@ def test_linear_act_sums_beyond_fp16(device, act):
     near(dx, dz @ w.double(), off @ w.double().abs())
     near(dw, dz.t() @ x.double(), off.t() @ x.double().abs() + 64 * U * (dz.abs().t() @ x.double().abs()))
     near(db, dz.sum(0), off.sum(0))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width', [7, 40, 513, 3000, 40000])
+@pytest.mark.parametrize('flat', [True, False])
+def test_token_logprobs_gradient_of_impossible_tokens(device, dtype, width, flat):
+    # rows whose token has a logit of -inf, is masked, or lies outside [0, C): the first
+    # two fall with the log of the sum, at the possible places alone, the last has no gradient
+    gen = torch.Generator().manual_seed(width)
+    logits = torch.randn(6, width + 3, generator=gen).to(device, dtype)[:, :width]
+    logits = logits.contiguous() if flat else logits
+    logits[:, 5] = -math.inf
+    mask = torch.ones(6, width, dtype=torch.bool, device=device)
+    mask[:, 2] = False
+    tokens = torch.tensor([5, 2, -1, width, 1 << 40, 3], device=device)
+    g, gh = torch.randn(2, 6, generator=gen).to(device)
+    for m, entropy in ((None, False), (mask, False), (mask, True)):
+        leaf = logits.detach().requires_grad_()
+        got = token_logprobs(leaf, tokens, mask=m)
+        d, = torch.autograd.grad([got.logprob, got.entropy], leaf, [g, gh * entropy])
+        ok = (logits > -math.inf) & (mask if m is not None else True)
+        logp = torch.where(ok, logits.double(), -math.inf).log_softmax(-1)
+        p, logp = logp.exp(), torch.where(ok, logp, 0.)
+        h = -(p * logp).sum(-1, keepdim=True)
+        one = torch.zeros_like(p)
+        one[5, 3] = 1.
+        if m is None:
+            one[1, 2] = 1.
+        glp = g.double().masked_fill((tokens < 0) | (tokens >= width), 0.).unsqueeze(-1)
+        want = glp * (one - p) - gh.double().unsqueeze(-1) * entropy * p * (logp + h)
+        # as in _lp_check; the logits range over some 10
+        off = U * (64 + 8 * 16) * 4 * (glp.abs() + gh.double().abs().unsqueeze(-1) * (1 + h))
+        near(d, want, off.expand_as(want))
+        assert bool((d[0] == 0)[5]) and bool((d[2:5] == 0).all()) or entropy
+        assert bool((d[:, 5] == 0).all())
