@@ -444,7 +444,8 @@ int linear_dtype(const Tensor& t, const char* name) {
 // leaves a tile's offsets in 32 bits.
 Rows product_rows_of(const Tensor& in) {
   if (in.size(-1) < 8) {
-    const Tensor wide = torch::constant_pad_nd(in, {0, 8 - in.size(-1)}, 0);
+    // the padding keeps another order of the dimensions, such as channels-last
+    const Tensor wide = torch::constant_pad_nd(in, {0, 8 - in.size(-1)}, 0).contiguous();
     return {wide, wide.numel() / 8, 8};
   }
   Rows r = rows_of(in);

@@ -1138,3 +1138,22 @@ def test_token_logprobs_gradient_of_impossible_tokens(device, dtype, width, flat
         near(d, want, off.expand_as(want))
         assert bool((d[0] == 0)[5]) and bool((d[2:5] == 0).all()) or entropy
         assert bool((d[:, 5] == 0).all())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', LOW)
+@pytest.mark.parametrize('k', [1, 3, 7, 8, 11])
+def test_linear_act_channels_last(device, dtype, k):
+    gen = torch.Generator().manual_seed(k)
+    w, b = torch.randn(9, k, generator=gen).to(device, dtype), torch.randn(9, generator=gen).to(device, dtype)
+    for shape, order in (((2, 5, 6, k), torch.channels_last), ((2, 3, 4, 5, k), torch.channels_last_3d)):
+        x = torch.randn(shape, generator=gen).to(device, dtype)
+        for n in (9, 3):                                  # rows of dy are narrow too
+            dy = torch.randn(*shape[:-1], n, generator=gen).to(device, dtype)
+            results = []
+            for fmt in (torch.contiguous_format, order):
+                leaves = [x.contiguous(memory_format=fmt).requires_grad_(), w[:n].clone().requires_grad_()]
+                y = linear_act(*leaves, b[:n], 'gelu')
+                results.append([y.detach(), *torch.autograd.grad(y, leaves, dy.contiguous(memory_format=fmt))])
+            for a, c in zip(*results):
+                assert a.shape == c.shape and torch.equal(a, c)
