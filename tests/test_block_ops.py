@@ -1157,3 +1157,17 @@ def test_linear_act_channels_last(device, dtype, k):
                 results.append([y.detach(), *torch.autograd.grad(y, leaves, dy.contiguous(memory_format=fmt))])
             for a, c in zip(*results):
                 assert a.shape == c.shape and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', LOW)
+def test_linear_act_gelu_far_below_zero(dtype):
+    # z is x itself. z * cdf is off by the fit of the cdf (4.2e-6 of it), by three
+    # roundings of z^2 / 2 in the exponent, and by some ten others
+    x = -torch.linspace(0.5, 12.5, 4096, dtype=torch.float64, device='cuda').reshape(256, 16).to(dtype)
+    w = torch.eye(16, dtype=dtype, device='cuda')
+    y = linear_act(x, w, None, 'gelu')
+    z = x.double().cpu()
+    want = (z * 0.5 * torch.special.erfc(z * -0.5 ** 0.5)).cuda()      # ndtr loses the tail by 1 + erf
+    z = z.cuda()
+    near(y, want, want.abs() * (4.2e-6 + (16 + 1.5 * z * z) * U))
