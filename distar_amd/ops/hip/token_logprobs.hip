@@ -39,6 +39,11 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// An exponent of 2 whose power is 0 in 32 bits. Where a power is multiplied with its
+// exponent, an infinite one is replaced by this, and so is a huge one, which a large
+// factor could take out of range: 0 times either is 0.
+constexpr float kFar = -256.f;
+
 __device__ __forceinline__ float exp2_(float y) {
   return __builtin_amdgcn_exp2f(y);
 }
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(LogProbs a) {
       for (int i = 0; i < V; ++i) {
         const float y = ((float)v[j][i] - m) * scale, e = exp2_(y);
         st.s += e;
-        st.u += e * fmaxf(y, -1e30f);       // e is 0 there
+        st.u += e * fmaxf(y, kFar);       // e is 0 there
       }
     }
     st.s = lanes_sum<TPR>(st.s);
@@ -318,14 +323,14 @@ void logprobs_kernel(LogProbs a) {
       for (int i = 0; i < V; ++i) {
         const float y = ((float)v[i] - m) * scale, e = exp2_(y);
         st.s += e;
-        st.u += e * fmaxf(y, -1e30f);       // e is 0 there
+        st.u += e * fmaxf(y, kFar);       // e is 0 there
       }
     };
     // the sums go over to a larger maximum; returns what to subtract
     auto raise = [&](float most) {
       const float m = fmaxf(st.m, most);
       const float by = m == -kInf ? 0.f : m;
-      const float d = fmaxf((st.m - by) * scale, -1e30f), f = exp2_(d);
+      const float d = fmaxf((st.m - by) * scale, kFar), f = exp2_(d);
       st.u = (st.u + d * st.s) * f;
       st.s *= f;
       st.m = m;
@@ -374,7 +379,7 @@ void logprobs_kernel(LogProbs a) {
     }
     {
       const float by = st.m == -kInf ? 0.f : st.m;
-      const float d = fmaxf((most - by) * scale, -1e30f), f = exp2_(d);
+      const float d = fmaxf((most - by) * scale, kFar), f = exp2_(d);
       st.u = lanes_sum<64>((st.u + d * st.s) * f);
       st.s = lanes_sum<64>(st.s * f);
     }
@@ -564,7 +569,7 @@ __device__ __forceinline__ float logit_grad(const RowGrad& r, float l, int c,
                                             float scale, float inv_t) {
   const float y = (l - r.m) * scale - r.log2sum;
   const float p = exp2_(y);
-  float d = -p * (r.glp + r.gh * (fmaxf(y, -1e30f) * kLn2 + r.h));
+  float d = -p * (r.glp + r.gh * (fmaxf(y, kFar) * kLn2 + r.h));
   d = y != y ? y : d;
   d += c == r.token ? r.glp : 0.f;
   return r.m == -kInf ? 0.f : d * inv_t;      // a row without any token

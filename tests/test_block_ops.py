@@ -1171,3 +1171,20 @@ def test_linear_act_gelu_far_below_zero(dtype):
     want = (z * 0.5 * torch.special.erfc(z * -0.5 ** 0.5)).cuda()      # ndtr loses the tail by 1 + erf
     z = z.cuda()
     near(y, want, want.abs() * (4.2e-6 + (16 + 1.5 * z * z) * U))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('width', [40, 3000])
+def test_token_logprobs_large_gradients_of_entropy(device, width):
+    # a scaled loss: places without probability stay without gradient
+    gen = torch.Generator().manual_seed(width)
+    logits = torch.randn(3, width, generator=gen).to(device)
+    logits[:, ::3] = -math.inf
+    logits[1, 1::3] = -1e9
+    grads = []
+    for scale in (1., 2. ** 34):
+        leaf = logits.clone().requires_grad_()
+        got = token_logprobs(leaf, torch.ones(3, dtype=torch.long, device=device))
+        grads.append(torch.autograd.grad(got.entropy.sum() * scale, leaf)[0])
+    assert bool(torch.isfinite(grads[0]).all())
+    assert torch.equal(grads[1], grads[0] * 2. ** 34)           # a power of two: no rounding
