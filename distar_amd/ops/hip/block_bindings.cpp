@@ -745,8 +745,6 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
       written.push_back(span_of(out));
     }
     g[i].out_dtype = dtype_of(out, "an output");
-    // autograd notices a change of what it has saved by the version
-    if (scale && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     g[i].in = in.data_ptr();
     g[i].out = out.data_ptr();
   }
@@ -766,6 +764,11 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
     for (size_t j = 0; j < i; ++j)
       TORCH_CHECK_VALUE(back[i].first.data_ptr() != back[j].first.data_ptr(),
                         "two of the tensors to be written share memory");
+  // autograd notices a change of what it has saved by the version: nothing behind here
+  // refuses the call
+  if (scale)
+    for (const Tensor& t : outs.has_value() ? *outs : grads)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   // neighbours in memory are one tensor to the kernels: a bucket's views end to end
   // are one entry instead of a thousand
   int count = 0;

@@ -1188,3 +1188,20 @@ def test_token_logprobs_large_gradients_of_entropy(device, width):
         grads.append(torch.autograd.grad(got.entropy.sum() * scale, leaf)[0])
     assert bool(torch.isfinite(grads[0]).all())
     assert torch.equal(grads[1], grads[0] * 2. ** 34)           # a power of two: no rounding
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_refused_clip_leaves_everything_as_it_was(device):
+    a = torch.randn(5, device=device, requires_grad=True)
+    b, c = torch.randn(5, device=device), torch.randn(5, device=device)
+    bad = [lambda: clip_grad_norm([b, c], 0.1, out=[b, c.long()]), lambda: clip_grad_norm([b, c], 0.1, out=[b, c[:3]]),
+           lambda: clip_grad_norm([b, c.long()], 0.1)]
+    if device == 'cuda':
+        bad += [lambda: clip_grad_norm([b, b], 0.1), lambda: clip_grad_norm([b, c.cpu()], 0.1),
+                lambda: clip_grad_norm([b, c], 0.1, out=[c, b])]
+    for call in bad:
+        y, kept = (a * b * c).sum(), (b.clone(), c.clone())
+        with pytest.raises((ValueError, TypeError)):
+            call()
+        assert torch.equal(b, kept[0]) and torch.equal(c, kept[1])
+        y.backward()                                       # b and c are as they were saved
