@@ -82,6 +82,17 @@ bool wants_grad(std::initializer_list<const OptTensor*> inputs) {
   return false;
 }
 
+// No kernel carries a forward-mode tangent on, and none may be lost in silence.
+void refuse_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what,
+                              " has no forward-mode derivative");
+}
+
+void refuse_tangents(std::initializer_list<const OptTensor*> inputs, const char* what) {
+  for (const auto* t : inputs)
+    if (t->has_value()) refuse_tangent(**t, what);
+}
+
 // Gradients come without a graph of their own: where one is being built, using
 // it raises an error.
 variable_list once(variable_list grads, const char* what) {
@@ -259,6 +270,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(Tensor x, OptTensor weight, OptTensor bias, double eps) {
   const OptTensor leaf = x;
+  refuse_tangents({&leaf, &weight, &bias}, "layer_norm");
   if (wants_grad({&leaf, &weight, &bias}))
     return LayerNorm::apply(x, OptTensor(), weight, bias, eps)[0];
   return layer_norm_fwd(x, {}, weight, bias, eps, false)[0];
@@ -267,6 +279,7 @@ Tensor layer_norm(Tensor x, OptTensor weight, OptTensor bias, double eps) {
 std::pair<Tensor, Tensor> add_layer_norm(Tensor x, Tensor residual, OptTensor weight,
                                          OptTensor bias, double eps) {
   const OptTensor leaf = x, other = residual;
+  refuse_tangents({&leaf, &other, &weight, &bias}, "add_layer_norm");
   if (wants_grad({&leaf, &other, &weight, &bias})) {
     const auto r = LayerNorm::apply(x, other, weight, bias, eps);
     return {r[0], r[1]};
@@ -422,6 +435,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_logprobs(
     Tensor logits, Tensor tokens, OptTensor mask, double temperature, int64_t top_k,
     int64_t ignore_index) {
   const OptTensor leaf = logits;
+  refuse_tangents({&leaf}, "token_logprobs");
   if (wants_grad({&leaf})) {
     const auto r = LogProbs::apply(logits, tokens, mask, temperature, top_k, ignore_index);
     if (!top_k) return {r[0], r[1], OptTensor(), OptTensor()};
@@ -668,6 +682,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 
 Tensor linear_act(Tensor x, Tensor weight, OptTensor bias, OptTensor residual, int64_t act) {
   const OptTensor leaf = x, w = weight;
+  refuse_tangents({&leaf, &w, &bias, &residual}, "linear_act");
   if (wants_grad({&leaf, &w, &bias, &residual}))
     return LinearAct::apply(x, weight, bias, residual, act);
   return linear_act_fwd(x, weight, bias, residual, act, false)[0];
@@ -710,6 +725,7 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
   for (int i = 0; i < listed; ++i) {
     Tensor in = grads[i];
     TORCH_CHECK_TYPE(in.layout() == torch::kStrided, "sparse tensors are not taken");
+    refuse_tangent(in, "a norm of gradients");
     check_device(in, first, "a tensor");
     g[i].in_dtype = dtype_of(in, "a tensor");
     g[i].numel = in.numel();
@@ -717,6 +733,7 @@ Tensor clip_grad_norm(std::vector<Tensor> grads,
     Tensor out = in;
     if (scale && outs.has_value()) {
       out = (*outs)[i];
+      refuse_tangent(out, "clipping");
       check_device(out, first, "an output");
       TORCH_CHECK_VALUE(out.sizes() == in.sizes(), "an output must be of its tensor's shape");
       const bool dense_out = out.is_non_overlapping_and_dense();

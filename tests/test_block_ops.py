@@ -1205,3 +1205,25 @@ def test_refused_clip_leaves_everything_as_it_was(device):
             call()
         assert torch.equal(b, kept[0]) and torch.equal(c, kept[1])
         y.backward()                                       # b and c are as they were saved
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    x, w, v = torch.randn(4, 8, device='cuda'), torch.randn(8, 8, device='cuda'), torch.randn(8, device='cuda')
+    tokens = torch.zeros(4, dtype=torch.long, device='cuda')
+    low = lambda t: t.bfloat16()  # noqa: E731
+    with fwd.dual_level():
+        dx, dw, dv = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, v))
+        lx, lw, lv = (fwd.make_dual(low(t), torch.ones_like(low(t))) for t in (x, w, v))
+        calls = [lambda: layer_norm(dx, v), lambda: layer_norm(x, dv), lambda: layer_norm(x, v, dv), lambda: add_layer_norm(x, dx),
+                 lambda: linear_act(lx, low(w)), lambda: linear_act(low(x), lw), lambda: linear_act(low(x), low(w), lv),
+                 lambda: linear_act(low(x), low(w), None, 'relu', lx), lambda: token_logprobs(dx, tokens),
+                 lambda: grad_norm([v, dx]), lambda: clip_grad_norm([v, dx], 1.),
+                 lambda: clip_grad_norm([v], 1., out=[dv])]
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+        assert torch.equal(layer_norm(x, v), layer_norm(fwd.unpack_dual(dx).primal, v))
+    layer_norm(x, v)
