@@ -109,9 +109,11 @@ class TransformerLayer(nn.Module):
         from ...ops.linear_act import LinearAct
         act = {nn.ReLU: 'relu', nn.GELU: 'gelu', nn.SiLU: 'silu',
                type(None): None}.get(type(activation), '?')
+        if act == 'gelu' and activation.approximate != 'none':
+            act = '?'
         if self.ln_type != 'pre' or self.dropout is not None or act == '?':
             raise ValueError('fused layers are pre-norm, without dropout, and have a relu, '
-                             f'gelu or silu; got {self.ln_type}, {self.dropout}, {activation}')
+                             f'exact gelu or silu; got {self.ln_type}, {self.dropout}, {activation}')
 
         def fused(linear, act):
             new = LinearAct(linear.in_features, linear.out_features, activation=act)

@@ -1227,3 +1227,11 @@ def test_forward_mode_tangents_are_refused():
                     call()
         assert torch.equal(layer_norm(x, v), layer_norm(fwd.unpack_dual(dx).primal, v))
     layer_norm(x, v)
+
+
+def test_fused_transformer_refuses_the_tanh_gelu():
+    from distar_amd.models.nn.transformer import Transformer
+    args = dict(input_dim=16, head_dim=8, hidden_dim=32, output_dim=16, head_num=2, layer_num=1, fused=True)
+    Transformer(**args, activation=torch.nn.GELU())
+    with pytest.raises(ValueError):
+        Transformer(**args, activation=torch.nn.GELU(approximate='tanh'))
