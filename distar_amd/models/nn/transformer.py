@@ -84,7 +84,8 @@ class TransformerLayer(nn.Module):
     """`fused`: a pre-norm layer without dropout on the block operators (same
     state dict): `ops/layer_norm.py` for the norms, `ops/linear_act.py` for the
     projection and the MLP, whose epilogues add the residual stream.  On a GPU
-    it needs autocast to bfloat16 or float16, the stream's type then."""
+    that takes autocast to bfloat16 or float16, the stream's type then; without
+    it the linear layers go through torch's float32 product."""
 
     def __init__(self, input_dim, head_dim, hidden_dim, output_dim, head_num,
                  mlp_num, dropout, activation, ln_type, fused=False):

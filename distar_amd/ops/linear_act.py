@@ -49,6 +49,10 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
     ext = hip_ext.maybe_ext(x)
     if ext is not None:
         return ext.linear_act(x, weight, bias, residual, ACTIVATIONS[activation])
+    return _composition(x, weight, bias, activation, residual)
+
+
+def _composition(x, weight, bias, activation, residual):
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f'x of shape {tuple(x.shape)} does not fit a weight of shape '
                          f'{tuple(weight.shape)}')
@@ -72,8 +76,9 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
 
 class LinearAct(nn.Linear):
     """`nn.Linear` (same state dict) with an activation and, when called with
-    one, a residual in the epilogue.  Under autocast it runs in autocast's type;
-    elsewhere x must be bfloat16 or float16 on a GPU."""
+    one, a residual in the epilogue.  Under autocast it runs in autocast's type.
+    The kernels take bfloat16 and float16; float32 on a GPU, as a model without
+    autocast has it, goes through torch's float32 product as in `nn.Linear`."""
 
     def __init__(self, in_features, out_features, bias=True, activation=None, **kwargs):
         super().__init__(in_features, out_features, bias=bias, **kwargs)
@@ -87,4 +92,6 @@ class LinearAct(nn.Linear):
             dtype = torch.get_autocast_dtype(x.device.type)
             x = x.to(dtype)
             residual = None if residual is None else residual.to(dtype)
+        if x.is_cuda and x.dtype == torch.float32:
+            return _composition(x, self.weight, self.bias, self.activation, residual)
         return linear_act(x, self.weight, self.bias, self.activation, residual)

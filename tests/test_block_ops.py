@@ -1235,3 +1235,29 @@ def test_fused_transformer_refuses_the_tanh_gelu():
     Transformer(**args, activation=torch.nn.GELU())
     with pytest.raises(ValueError):
         Transformer(**args, activation=torch.nn.GELU(approximate='tanh'))
+
+
+@pytest.mark.gpu
+def test_fused_transformer_in_float32():
+    # as an actor without a batch server and a learner without autocast run it
+    from distar_amd.models.nn.transformer import Transformer
+    torch.manual_seed(0)
+    args = dict(input_dim=48, head_dim=128, hidden_dim=160, output_dim=96, head_num=2, layer_num=2)
+    plain, fused = Transformer(**args).cuda(), Transformer(**args, fused=True).cuda()
+    fused.load_state_dict(plain.state_dict())
+    x = torch.randn(3, 20, 48, device='cuda')
+    mask = torch.arange(20, device='cuda') < torch.tensor([[20], [7], [1]], device='cuda')
+    dy = torch.randn(3, 20, 96, device='cuda')
+    want, got = plain(x, mask), fused(x, mask)
+    assert got.dtype == torch.float32
+    ref, grads = (torch.autograd.grad(y, list(m.parameters()), dy) for y, m in ((want, plain), (got, fused)))
+    # sums of up to 256 products, some twenty of them in a row, 32-bit; a relu whose input
+    # lies within that noise may change sides, as in the test of the 16-bit stream
+    noise = 20 * 16 * U
+    flips = math.sqrt(5 * 0.8 * noise)
+    for a, b, most in zip([got, *grads], [want, *ref], [noise] + [noise + flips] * len(grads)):
+        assert torch.linalg.vector_norm((a - b).double()) <= most * torch.linalg.vector_norm(b.double()) + 1e-6
+    module = LinearAct(48, 8, activation='silu').cuda()
+    torch.testing.assert_close(module(x), torch.nn.functional.silu(torch.nn.functional.linear(x, module.weight, module.bias)))
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        assert module(x).dtype == torch.bfloat16
