@@ -71,7 +71,9 @@ def _composition(x, weight, bias, activation, residual):
                              f'{(*x.shape[:-1], weight.shape[0])}')
         if residual.dtype != x.dtype:
             raise TypeError(f'residual is {residual.dtype}, but x is {x.dtype}')
-    return _eager(x, weight, bias, activation, residual)
+    # autocast would take the product's sums out of 32 bits
+    with torch.autocast(x.device.type, enabled=False):
+        return _eager(x, weight, bias, activation, residual)
 
 
 class LinearAct(nn.Linear):

@@ -1261,3 +1261,20 @@ def test_fused_transformer_in_float32():
     torch.testing.assert_close(module(x), torch.nn.functional.silu(torch.nn.functional.linear(x, module.weight, module.bias)))
     with torch.autocast('cuda', dtype=torch.bfloat16):
         assert module(x).dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_linear_act_sums_stay_32_bit_under_autocast(device, monkeypatch):
+    if device == 'cuda':
+        monkeypatch.setenv('DISTAR_AMD_DISABLE_HIP', '1')
+    gen = torch.Generator().manual_seed(1)
+    x, w = torch.randn(30, 64, generator=gen).to(device).bfloat16(), torch.randn(9, 64, generator=gen).to(device)
+    b, dy = torch.randn(9, generator=gen).to(device), torch.randn(30, 9, generator=gen).to(device).bfloat16()
+    results = []
+    for autocast in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        with torch.autocast(device, dtype=torch.bfloat16, enabled=autocast):
+            y = linear_act(*leaves, 'gelu')
+        results.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    for a, c in zip(*results):
+        assert a.dtype == c.dtype and torch.equal(a, c)
