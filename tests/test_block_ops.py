@@ -1278,3 +1278,29 @@ def test_linear_act_sums_stay_32_bit_under_autocast(device, monkeypatch):
         results.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
     for a, c in zip(*results):
         assert a.dtype == c.dtype and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_layer_norm_of_very_wide_rows_closely():
+    # A block of 1024 threads adds up a row, n values each. Roundings of either sign add up
+    # to 6 sqrt(n) of them but for 4 sums in 10^8 (Hoeffding's bound for n independent ones
+    # of at most u each gives 2 exp(-18)), so a mean is off by that many u of the mean
+    # magnitude, where the worst case, n, would be as large as the values themselves.
+    width = 2 ** 25 + 9
+    gen = torch.Generator('cuda').manual_seed(1)
+    x, dy = torch.randn(2, 2, width, generator=gen, device='cuda') + 0.25
+    w, b = torch.randn(2, width, generator=gen, device='cuda')
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    ref = _ln_reference(x, w, b, 1e-5, dy)
+    e = (6 * math.sqrt(width / 1024) + 32) * U
+    assert e < 1e-4
+    size = x.double().abs().mean(-1, keepdim=True)
+    h_off = e * (ref['r'] * size + ref['h'].abs())             # of the mean, and of 1 / the deviation
+    near(y, ref['y'], h_off * w.double().abs() + 4 * U * (ref['y'].abs() + b.double().abs()))
+    g = dy.double() * w.double()
+    m1, m2 = g.abs().mean(-1, keepdim=True), (g * ref['h']).abs().mean(-1, keepdim=True)
+    near(dx, ref['dx'], ref['r'] * (e * (2 * m1 + 2 * m2 * (1 + ref['h'].abs()) + g.abs()) + h_off * m2) + 8 * U * g.abs() * ref['r'])
+    near(dw, ref['dw'], (dy.double().abs() * h_off).sum(0) + 4 * U * ref['dw_abs'])
+    near(db, ref['db'], 2 * U * ref['db_abs'])
