@@ -431,7 +431,6 @@ __global__ __launch_bounds__(WI * WJ * 64, BI * BJ < 128 * 128 ? 4 : 2)
 void product_kernel(Product a, Tiles map) {
   constexpr int NT = WI * WJ * 64;
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
-  constexpr int kReads = (PT ? 2 : 1) * FI + (QT ? 2 : 1) * FJ;
   constexpr int kPBytes = Tile<BI, PT, kSR>::bytes;
   constexpr int kBytes = kPBytes + Tile<BJ, QT, kSR>::bytes;
   using P = Staged<T, BI, PT, NT>;
@@ -778,13 +777,13 @@ void product_few_kernel(Product a) {
 
 constexpr int kActRows = 4;           // rows of a thread under way together
 
-// 32 threads take 8 columns each, 8 rows at a time. NARROW: fewer than 8 columns.
 template <typename T>
 __device__ __forceinline__ void put_dbias(const ActBwd& a, int64_t c, float v) {
   if (a.dbias_f32) ((float*)a.dbias)[c] = v;
   else ((T*)a.dbias)[c] = (T)v;
 }
 
+// 32 threads take 8 columns each, 8 rows at a time. NARROW: fewer than 8 columns.
 template <typename T, int ACT, bool NARROW>
 __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwd a) {
   __shared__ float part[8][257];

@@ -127,7 +127,6 @@ constexpr int kList = 1024;         // alternatives' candidates of a block
 template <int TPR>
 struct Shared {
   static constexpr int waves = TPR > 64 ? TPR / 64 : 1;
-  static constexpr int rows = TPR > 64 ? 1 : 256 / TPR;
   static constexpr int list = kList / (TPR > 64 ? 1 : 4);   // of a row or wave
   float most[waves];
   Stat stat[waves];
