@@ -2,8 +2,11 @@
 
 `grad_norm` and `clip_grad_norm` take float32, bfloat16 and float16 tensors in
 any mix, of any sizes and strides, and keep the norm on the device: nothing in
-them waits for the GPU.  Sums are 64-bit and in a fixed order, so the norm is
-the same each time and does not overflow before the norm itself does.
+them waits for the GPU.  Sums are 64-bit but for runs of eight, so the norm does
+not overflow before it has to.  Their order is fixed by the tensors' sizes and
+places in memory: the same tensors give the same norm each time, equal ones in
+other places may differ in its last bit.  Replicas that have to agree to the bit
+take the norm of one of them, or one bucket laid out alike.
 `utils/grad_clip.py` offers them as ``type: global_norm``.
 
 On a GPU the kernels in `ops/hip/grad_norm.hip` run; CPU tensors (and

@@ -10,7 +10,10 @@
 // is copied to the device and a captured graph keeps its own. A block takes one
 // chunk of one tensor and leaves one partial sum; a last block adds those up in a
 // fixed order. Sums over more than 8 elements are 64-bit, so they neither overflow
-// nor drift.
+// nor drift. Which elements share a run, and so the sums' last digits, depends on where
+// the tensors lie: chunks begin at 16-byte boundaries, and neighbours are one tensor.
+// The same call on the same memory gives the same norm; equal values that lie
+// otherwise may differ in its last bit.
 //
 // Tensors may start at any element (views of a flat bucket do). A chunk is cut
 // where 16-byte accesses are aligned: to what is read in the norm, to what is

@@ -2,7 +2,8 @@
 none / max_norm (EMA-normalized) / momentum_norm (per-param EMA) /
 clip_value (second-moment clamp) / clip_const / pytorch_norm, and global_norm:
 the clip of pytorch_norm for gradients of mixed types, strides and norms 1, 2
-and inf, with sums that come out the same each time (`ops/grad_norm.py`).
+and inf, with sums that come out the same each time for the same gradients in
+the same memory (`ops/grad_norm.py`).
 
 On GPU the norm computations use torch's fused multi-tensor paths
 (`torch.nn.utils.clip_grad_norm_` with foreach=True) — one kernel per dtype
