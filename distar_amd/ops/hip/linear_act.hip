@@ -19,10 +19,11 @@
 // dz is rounded to that type, because both products take no wider one.
 //
 // The matrix cores bound long r, memory the rest. 16384 x 4096 by 2048 fp16 with
-// gelu, residual and z kept: 328 us, 838 TFLOP/s (231 us, 1190 TFLOP/s, without an
-// epilogue: 256 x 256 tiles fill a compute unit, so nothing hides their 200 MB);
-// dz 38 us, dx 292 us (942), dW 249 us (1104) and 14 us to join its two parts.
-// 32768 x 997 by 256 bf16 with relu: 40 us, dz and db 12 + 4, dx 35, dW 34 + 7.
+// gelu, residual and z kept, within a pass: 337 us, 817 TFLOP/s (on its own 309 us, and
+// 248 us, 1110 TFLOP/s, without an epilogue: 256 x 256 tiles fill a compute unit, so
+// nothing hides their 268 MB); dz 45 us, 5.9 TB/s, dx 292 us (942), dW 244 us (1126)
+// and 14 us to join its two parts. 32768 x 997 by 256 bf16 with relu: 39 us, dz and db
+// 11 + 4, dx 35, dW 34 + 7.
 #include <type_traits>
 
 #include "block_common.h"
@@ -872,10 +873,11 @@ bool few(const Product& a) {
 }
 
 // Tiles of 256 x 256, of which one fills a compute unit, need 1024 r to outweigh
-// their first loads (bare, 16384 x 1024 by 4096 takes 164 us by tiles of 128, 151 us
-// by these; 32768 x 1000 by 256 34 and 52) and 2048 where nothing hides an activation
-// behind them (with gelu 183 and 192; 8192 x 2048 by 2048 86 and 75), and either
-// enough of them for all compute units or enough r to share a tile among two blocks.
+// their first loads (bare, 16384 x 1024 by 4096 takes 156 us by tiles of 128, 149 us
+// by these; 32768 x 1000 by 256 31 and 48) and 2048 where nothing hides an activation
+// behind them (with gelu 181 and 205; 8192 x 2048 by 2048 86 and 82, with a residual
+// and z kept 104 and 91), and either enough of them for all compute units or enough r
+// to share a tile among two blocks.
 bool large(const Product& a) {
   const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);
   return direct(a) && ((a.r >= (a.act ? 2048 : 1024) && tiles >= 192) || (a.r >= 4096 && tiles >= 96));
@@ -890,10 +892,11 @@ struct Plan {
 // r take where it is alone on its compute unit (at least `alone`) and for each
 // block that shares it (`shared`), and by the joining of parts: a launch, 8 bytes
 // of traffic for each value of a part, and a wait for each batch of parts. The
-// figures, in us, are fitted to 1000 timed products of 16 to 131072 rows, of which
-// the choice is 1% slower than the best of each. (In us, as chosen and by tiles of
-// 128 with parts for two blocks a compute unit: 512 x 1024 by 1024 10.5 and 20.6,
-// 2048 x 997 by 256 10.4 and 24.5, 16384 x 256 by 256 9.4 and 26.5.)
+// figures, in us, are fitted to timed products. Of 162 products of 1 to 131072 rows
+// (profiles/block_ops_linear_tiles.csv: each with either side and every number of
+// parts) the choice is on average 0.7% slower than the best, at worst 21%. (In us, as
+// chosen and by tiles of 128 with parts for two blocks a compute unit: 512 x 1024 by
+// 1024 10.7 and 26.4, 2048 x 997 by 256 10.0 and 24.7, 16384 x 256 by 256 9.1 and 27.1.)
 Plan plan(const Product& a) {
   if (large(a)) {
     const int64_t tiles = ceil_div(a.i, 256) * ceil_div(a.j, 256);

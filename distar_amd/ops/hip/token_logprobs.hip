@@ -697,13 +697,14 @@ void fwd_as(const LogProbs& a, hipStream_t stream) {
     logprobs_kernel<T, TPR, false, kBatch><<<grid, TPR > 64 ? TPR : 256, 0, stream>>>(a);
 }
 
-// Rows of up to 128 runs lie in registers (65536 x 513 bf16: 17 us, 52 us by a wave
-// that runs through the row). Longer ones take a wave up to 256 runs (8192 x 2000:
-// 10 us, 47 us with 256 threads; of at most 128 runs, with alternatives, by a kernel
-// that holds no second batch: 65536 x 513 with a mask and 5 of them 84 us, 148 us by
-// the general one), then 256 threads (2048 x 24320: 29 us, 38 us with
-// 512), and 512 where rows are too few to fill the chip (33 x 24320 fp32 with 20
-// alternatives: 12.3 us, 14.6 us with 256).
+// Rows of up to 128 runs lie in registers (65536 x 513 bf16: 16 us, 52 us by a wave
+// that runs through the row). 49 to 64 runs share the variant of 80: 65536 x 512 bf16
+// takes 15.0 us, 13.9 with a variant of its own, and 21.3 and 20.7 with a mask. Longer
+// ones take a wave up to 256 runs (8192 x 2000: 10 us, 47 us with 256 threads; of at
+// most 128 runs, with alternatives, by a kernel that holds no second batch: 65536 x
+// 513 with a mask and 5 of them 84 us, 148 us by the general one), then 256 threads
+// (2048 x 24320: 29 us, 38 us with 512), and 512 where rows are too few to fill the
+// chip (33 x 24320 fp32 with 20 alternatives: 12.3 us, 14.6 us with 256).
 template <typename T>
 void fwd(const LogProbs& a, hipStream_t stream) {
   const int n = (a.width + Width<T>::v - 1) / Width<T>::v;    // runs of 16 bytes
