@@ -19,6 +19,11 @@ from . import hip_ext
 ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
 
 
+def _autocasts(x):
+    kind = x.device.type
+    return torch.amp.is_autocast_available(kind) and torch.is_autocast_enabled(kind)
+
+
 def _eager(x, weight, bias, activation, residual):
     wide = torch.promote_types(x.dtype, torch.float32)
     z = x.to(wide) @ weight.to(x.dtype).to(wide).t()
@@ -71,6 +76,8 @@ def _composition(x, weight, bias, activation, residual):
                              f'{(*x.shape[:-1], weight.shape[0])}')
         if residual.dtype != x.dtype:
             raise TypeError(f'residual is {residual.dtype}, but x is {x.dtype}')
+    if not _autocasts(x):
+        return _eager(x, weight, bias, activation, residual)
     # autocast would take the product's sums out of 32 bits
     with torch.autocast(x.device.type, enabled=False):
         return _eager(x, weight, bias, activation, residual)
@@ -90,7 +97,7 @@ class LinearAct(nn.Linear):
         self.activation = activation
 
     def forward(self, x, residual=None):
-        if torch.is_autocast_enabled(x.device.type):
+        if _autocasts(x):
             dtype = torch.get_autocast_dtype(x.device.type)
             x = x.to(dtype)
             residual = None if residual is None else residual.to(dtype)

@@ -1304,3 +1304,10 @@ def test_layer_norm_of_very_wide_rows_closely():
     near(dx, ref['dx'], ref['r'] * (e * (2 * m1 + 2 * m2 * (1 + ref['h'].abs()) + g.abs()) + h_off * m2) + 8 * U * g.abs() * ref['r'])
     near(dw, ref['dw'], (dy.double().abs() * h_off).sum(0) + 4 * U * ref['dw_abs'])
     near(db, ref['db'], 2 * U * ref['db_abs'])
+
+
+def test_linear_act_of_meta_tensors():
+    # a device that autocast does not know
+    x, module = torch.empty(4, 8, device='meta', requires_grad=True), LinearAct(8, 3, activation='gelu', device='meta')
+    for y in (linear_act(x, module.weight, module.bias, 'gelu'), module(x)):
+        assert y.shape == (4, 3) and y.device.type == 'meta'
